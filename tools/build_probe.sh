@@ -9,7 +9,7 @@ build() {
   tag=$1; shift
   for f in abi_misc elementwise gemm_bf16 flash_attn lmhead_confidence confidence_logits sampler; do
     if [ "$f" = gemm_bf16 ] || [ ! -f /tmp/probe_obj/$f.o ]; then
-      hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I. -Wno-unused-function -ffp-contract=off -DCODA_CLOCK_PROBE $@ -c $f.hip -o /tmp/probe_obj/$f$([ "$f" = gemm_bf16 ] && echo "_$tag").o
+      hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I"$ROOT/include" -I. -Wno-unused-function -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -DCODA_CLOCK_PROBE $@ -c $f.hip -o /tmp/probe_obj/$f$([ "$f" = gemm_bf16 ] && echo "_$tag").o
     fi
   done
   hipcc -shared -fPIC --offload-arch=gfx950 /tmp/probe_obj/abi_misc.o /tmp/probe_obj/elementwise.o /tmp/probe_obj/gemm_bf16_$tag.o /tmp/probe_obj/flash_attn.o \
