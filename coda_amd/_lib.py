@@ -10,6 +10,8 @@ LIB_PATH = os.path.join(_HERE, "csrc", "libcoda_hip.so")
 EPI_PLAIN, EPI_RESIDUAL, EPI_SWIGLU, EPI_F32 = 0, 1, 2, 3
 GEMM_NARROW_STORES = 1
 ALG_IDS = {"maskgit_plus": 0, "topk_margin": 1, "entropy": 2}
+CACHE_BF16, CACHE_E4M3 = 0, 1
+APPEND_STEPWISE = 1
 ERRORS = {-1: "CODA_ERR_SHAPE", -2: "CODA_ERR_ALIGN", -3: "CODA_ERR_LAUNCH", -4: "CODA_ERR_ARG"}
 
 _p, _i, _ll, _f, _ull = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_ulonglong
@@ -43,6 +45,11 @@ SIGNATURES = {
     "coda_scatter_rows": (_i, [_p, _ll, _p, _i, _p, _ll, _i, _i, _p]),
     "coda_gemm_bf16_counted":(_i, [_p, _ll, _p, _p, _ll, _p, _ll, _i, _i, _i, _p]),
     "coda_select_threshold": (_i, [_p, _p, _p, _i, _i, _i, _ll, _i, _f, _p, _p]),
+    "coda_paged_append": (_i, [_p, _ll, _p, _ll, _p, _p, _p, _p, _i, _p, _p, _i, _i, _p, _ll, _i, _p, _p, _ll, _i, _i, _i, _f, _f, _i,
+                               _i, _f, _i, _p]),
+    "coda_paged_attn_workspace_bytes": (_ll, [_i, _i, _i, _i, _i]),
+    "coda_paged_attn": (_i, [_p, _ll, _p, _ll, _p, _p, _p, _i, _i, _p, _ll, _i, _p, _p, _ll, _i, _i, _i, _f, _f, _i, _i, _i, _f, _i, _p,
+                             _ll, _p]),
     "coda_origin_transfer": (_i, [_p, _p, _p, _p, _i, _p, _ull, _f, _p]),
 }
 

@@ -1,0 +1,931 @@
+// Attention of new tokens over a paged key/value cache, head_dim 128.
+//
+//     out_i = sum_j softmax_j(scale q_i . K_j) V_j over the keys j < lim(i) of the token's sequence
+//
+// One pass over the keys with a running maximum and sum (in log2 units); the keys are cut into `nsplit` ranges where there
+// are too few rows to fill the chip, and a second kernel joins the ranges' (maximum, sum, unnormalised output) triples in
+// fp32, in a fixed order.
+//
+// Rows.  The g = n_q / n_kv query heads of a key/value head read the same keys, so a sequence of n tokens is n g ROWS per
+// key/value head (row r = token r / g, head r % g) and tiles are cut from those: one token of a g = 2 model is two rows of one
+// tile, a block of 32 tokens is 64.
+//
+// MFMA orientation (v_mfma_f32_32x32x16_bf16), as in flash_attn.hip: S^T[key][row] = K Q^T with K rows from LDS and Q^T in
+// registers, so a lane holds one row's scores and the accumulator registers are directly the B operand of
+// O^T[d][row] += V^T P^T, whose A operand is read from LDS with the transposing ds_read_b64_tr_b16.
+// LDS image of a K or V tile: 256 B a key (bf16 also for e4m3 pages: the conversion is exact), 16-byte chunk ch of key r at
+// ch ^ swz(r): free of bank conflicts for both kinds of read.
+//
+// Pages reach LDS through registers (global loads of the NEXT tile fly under the current tile's products): keys of a tile
+// may lie on different pages, e4m3 is converted on the way, and keys beyond the sequence or on an invalid page are zeroed
+// on the way, so that whatever their slots hold (infinities, NaN) cannot reach the sums through 0 * x.
+#include "paged_common.h"
+#include <type_traits>
+
+using namespace paged;
+
+namespace {
+
+constexpr float RESCALE_THR = 6.0f;            // log2 units: weights stay below 2^6 between rescales
+constexpr int MAX_SPLITS = 256;
+
+struct AttnArgs {
+    const char* q; long long ldq_b;
+    char* out; long long ldo_b;
+    const int* seq_start; const int* pos0; const int* kv_len;
+    int B, T, max_kv;
+    Pages pg;
+    const char* k; const char* v;
+    int n_q, n_kv, g;
+    FastDiv gdiv;
+    int mask_block;
+    float scale_log2e, v_scale;
+    int nslots, nsplit, split_len;
+    float* po; float* pml;                     // partial outputs [nsplit][T n_q][128] and (maximum, sum) [nsplit][T n_q][2]
+};
+
+__device__ __forceinline__ int swz(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+
+typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+
+// A tile of `R` rows of one sequence: tile slots are numbered so that sequence b owns floor(start_b g / R) + b onwards, which
+// needs no prefix sum over the sequences and leaves each at least ceil(n g / R) slots (a slot beyond its rows is idle).
+struct TileRows {
+    int b, s0, n;        // sequence, its first token row, its tokens
+    int r0, rows;        // first row of the tile, rows of the sequence
+};
+
+template <int R>
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, int slot, TileRows& t) {
+    auto first = [&](int i) { return (long long)clamp_start(a.seq_start, i, a.T) * a.g / R + i; };
+    t.b = wave_search(a.B, slot, first);
+    if (t.b < 0) return false;
+    t.s0 = clamp_start(a.seq_start, t.b, a.T);
+    t.n = clamp_start(a.seq_start, t.b + 1, a.T) - t.s0;
+    t.rows = t.n * a.g;
+    const long long r0 = (slot - first(t.b)) * R;
+    t.r0 = (int)r0;
+    return r0 < t.rows;
+}
+
+// Keys that token i of the sequence sees: all of its kv_len, or those before the end of the token's mask block.
+struct Limits {
+    int kv; long long pos0;
+};
+
+__device__ __forceinline__ Limits load_limits(const AttnArgs& a, int b) {
+    Limits l;
+    l.kv = min(max(a.kv_len[b], 0), a.max_kv);
+    l.pos0 = a.mask_block ? a.pos0[b] : 0;
+    return l;
+}
+
+__device__ __forceinline__ int limit_of(const AttnArgs& a, const Limits& l, int token) {
+    if (a.mask_block == 0) return l.kv;
+    const long long p = l.pos0 + token;
+    if (p < 0) return 0;
+    const long long end = ((long long)((unsigned int)p / (unsigned int)a.mask_block) + 1) * a.mask_block;
+    return (int)min((long long)l.kv, end);
+}
+
+// byte offset of key `key` (of this sequence and head) inside the cache; ok = false for keys outside [0, end) and bad pages
+struct KeyAt {
+    size_t off; bool ok;
+};
+
+__device__ __forceinline__ int page_entry(const AttnArgs& a, const int* table, int key, int end) {
+    return key < end ? table[fast_div(a.pg.page, key)] : -1;
+}
+
+__device__ __forceinline__ KeyAt key_at(const AttnArgs& a, int entry, int key) {
+    KeyAt k;
+    k.ok = (unsigned)entry < (unsigned)a.pg.num_pages;
+    const int slot = key - fast_div(a.pg.page, key) * (int)a.pg.page.d;
+    k.off = k.ok ? (size_t)entry * a.pg.page_stride_b + (size_t)slot * a.pg.row_b : 0;
+    return k;
+}
+
+__device__ __forceinline__ size_t shfl_size(size_t v, int src) {
+    const unsigned lo = __shfl((int)(unsigned)v, src, 64), hi = __shfl((int)(unsigned)(v >> 32), src, 64);
+    return ((size_t)hi << 32) | lo;
+}
+
+// Source addresses of a tile's 1 KiB pieces (4 bf16 or 8 e4m3 keys each).  Pages of a multiple of 16 keys (G16): any 16 aligned
+// keys lie on one page, one after the other, so a group of 16 has ONE wave-uniform base, its pieces are whole contiguous KiB at
+// constant offsets from it and the address costs no vector instruction.  Other page sizes: lane l looks key l of the tile up and the
+// loads fetch their key's offset from it by shuffles.
+// A wave fetches pieces first, first + STRIDE, ... (NP of them).
+template <int KEYS, int NP, int STRIDE, bool F8, bool G16>
+struct TileSource {
+    static constexpr int GROUPS = KEYS / 16;
+    static constexpr int PROWS = F8 ? 8 : 4;
+    static constexpr int SUB = F8 ? 8 : 16;    // lanes per key
+    int first;
+    size_t base[G16 ? NP : 1];                 // G16: of each piece's group (uniform); else: of key lane & (KEYS - 1)
+    unsigned long long ok;                     // keys that exist
+    int entry[G16 ? GROUPS : 1], mine[G16 ? NP : 1];      // page numbers of the tile looked up last: of every group, of this wave's pieces
+
+    __device__ __forceinline__ int group_key(int i) const { return ((i * STRIDE + first) * PROWS) & ~15; }
+    __device__ __forceinline__ void look_up(const AttnArgs& a, const int* table, int key0, int end) {
+        if (G16) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) entry[g] = page_entry(a, table, key0 + 16 * g, end);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) mine[i] = page_entry(a, table, key0 + group_key(i), end);
+        } else {
+            entry[0] = page_entry(a, table, key0 + (int)(threadIdx.x & (KEYS - 1)), end);
+        }
+    }
+    // page numbers -> offsets, for the tile that look_up was last called for
+    __device__ __forceinline__ void resolve(const AttnArgs& a, int key0, int end) {
+        if (G16) {
+            ok = 0;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const int live = (unsigned)entry[g] < (unsigned)a.pg.num_pages ? min(max(end - key0 - 16 * g, 0), 16) : 0;
+                ok |= (unsigned long long)((1u << live) - 1u) << (16 * g);
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i) base[i] = key_at(a, mine[i], key0 + group_key(i)).off;
+        } else {
+            const KeyAt at = key_at(a, entry[0], key0 + (int)(threadIdx.x & (KEYS - 1)));
+            ok = __ballot(at.ok);
+            if (KEYS < 64) ok &= (1ull << (KEYS & 63)) - 1;
+            base[0] = at.off;
+        }
+    }
+    // this lane's 16 bytes of the wave's piece i
+    __device__ __forceinline__ size_t at(int i) const {
+        const int lane = threadIdx.x & 63, key = (i * STRIDE + first) * PROWS;
+        if (G16) return base[i] + (size_t)((key & 15) * (16 * SUB) + lane * 16);
+        return shfl_size(base[0], key + lane / SUB) + (lane % SUB) * 16;
+    }
+};
+
+// four e4m3 bytes -> four bf16 (exact: three mantissa bits, exponents within bf16's)
+__device__ __forceinline__ u32x2_t bf16_of_e4m3(unsigned int w) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    u32x2_t o;
+    o[0] = pack_bf16x2(lo[0], lo[1]);
+    o[1] = pack_bf16x2(hi[0], hi[1]);
+    return o;
+}
+
+// bf16 infinities and NaN of a 16-byte piece set to zero; true if there were any
+__device__ __forceinline__ bool drop_nonfinite(u32x4_t& v) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool lo = (v[i] & 0x7f80u) == 0x7f80u, hi = (v[i] & 0x7f800000u) == 0x7f800000u;
+        if (lo) v[i] &= 0xffff0000u;
+        if (hi) v[i] &= 0x0000ffffu;
+        any |= lo | hi;
+    }
+    return any;
+}
+
+// A tile that some row sees only in part holds values of keys that other rows must not feel, and the products cannot skip
+// them: 0 * inf = NaN.  Staging such a tile drops its infinities and NaN from the LDS image; if there were any, this finds
+// the outputs they belong to: those features of the rows that do see their key come out as NaN.  Bit 16 db + i of the answer
+// stands for accumulator register i of feature block db.  Rare, and slow on purpose: a rolled loop that needs no registers.
+template <bool F8>
+__device__ __forceinline__ unsigned long long find_nonfinite(const AttnArgs& a, const int* table, size_t head_off, int key0, int nkeys,
+                                                             int end, int lim, int half) {
+    unsigned long long bits = 0;
+#pragma unroll 1
+    for (int j = 0; j < nkeys; ++j) {
+        const int key = key0 + j;
+        const KeyAt at = key_at(a, page_entry(a, table, key, end), key);
+        if (key >= end || !at.ok || key >= lim) continue;
+        const char* p = a.v + head_off + at.off;
+#pragma unroll 1
+        for (int e = 0; e < 64; ++e) {
+            const int d = 32 * (e >> 4) + (e & 3) + 8 * ((e >> 2) & 3) + 4 * half;
+            const bool bad = F8 ? (((const unsigned char*)p)[d] & 0x7f) == 0x7f : (((const unsigned short*)p)[d] & 0x7f80) == 0x7f80;
+            if (bad) bits |= 1ull << e;
+        }
+    }
+    return bits;
+}
+
+__device__ __forceinline__ void poison(f32x16_t (&o)[4], unsigned long long bits) {
+    if (!__any(bits != 0)) return;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((bits >> (16 * db + i)) & 1) o[db][i] = __builtin_nanf("");
+}
+
+// output row of a tile row: token row and head
+struct RowAt {
+    int token, head;
+};
+
+__device__ __forceinline__ RowAt row_at(const AttnArgs& a, const TileRows& t, int kvh, int r) {
+    const int i = fast_div(a.gdiv, r);
+    return {t.s0 + i, kvh * a.g + (r - i * a.g)};
+}
+
+// one row's 8 consecutive outputs (d0..): normalised bf16 to `out`, or fp32 partials
+__device__ __forceinline__ u32x4_t pack8(const float (&f)[8]) {
+    u32x4_t v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+    return v;
+}
+
+// Writes a lane's 16 bytes of a K and of a V piece into the tile images (bf16 rows of 256 B, chunk ch of key r at ch ^ swz(r)).
+// PART: keys that do not exist become zeros in the V image, and so do infinities and NaN; true if there were any of those.
+template <bool F8>
+struct ImageWriter {
+    int row0, at0;                             // key within the piece, and its byte offset with the swizzle's lane-dependent part
+    __device__ __forceinline__ explicit ImageWriter(int lane) {
+        row0 = F8 ? lane >> 3 : lane >> 4;
+        const int ch = F8 ? 2 * (lane & 7) : lane & 15;
+        at0 = row0 * 256 + ((ch ^ ((row0 & 3) << 2)) << 4);
+    }
+    template <bool PART>
+    __device__ __forceinline__ bool put(char* kimg, char* vimg, int piece, const u32x4_t& k, const u32x4_t& v, unsigned long long ok) const {
+        bool dropped = false;
+        const bool live = !PART || ((ok >> (piece * (F8 ? 8 : 4) + row0)) & 1);
+        const u32x4_t zero = {0, 0, 0, 0};
+        if (F8) {
+            // key 8 piece + row0: swz's low part is (2 piece + (row0 >> 2)) & 3
+            const int x = (((2 * piece) & 3) ^ (row0 >> 2)) << 4;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const u32x2_t k0 = bf16_of_e4m3(k[2 * j]), k1 = bf16_of_e4m3(k[2 * j + 1]);
+                const u32x2_t v0 = bf16_of_e4m3(v[2 * j]), v1 = bf16_of_e4m3(v[2 * j + 1]);
+                u32x4_t vw = {v0[0], v0[1], v1[0], v1[1]};
+                if (PART) {
+                    if (!live) vw = zero;
+                    dropped |= drop_nonfinite(vw);
+                }
+                const int at = piece * 2048 + (at0 ^ x ^ (j << 4));
+                *(u32x4_t*)(kimg + at) = (u32x4_t){k0[0], k0[1], k1[0], k1[1]};
+                *(u32x4_t*)(vimg + at) = vw;
+            }
+        } else {
+            // key 4 piece + row0: swz's low part is piece & 3
+            u32x4_t vw = v;
+            if (PART) {
+                if (!live) vw = zero;
+                dropped = drop_nonfinite(vw);
+            }
+            const int at = piece * 1024 + (at0 ^ ((piece & 3) << 4));
+            *(u32x4_t*)(kimg + at) = k;
+            *(u32x4_t*)(vimg + at) = vw;
+        }
+        return dropped;
+    }
+};
+
+// MFMA fragments out of the images.
+//   K (A operand of S^T, 32 keys x 16 features): lane -> key 32 k2 + (lane & 31), chunk 2 ks + (lane >> 5)
+//   V^T (A operand of O^T, 32 features x 16 keys): the transposing read; lane i16 = lane & 15 addresses key tq = i16 >> 2 of
+//   the quad 16 st + 4 h (and + 8), chunk 4 db + 2 ((lane >> 4) & 1) + ((i16 & 3) >> 1), byte 8 (i16 & 1)
+// The offsets are recomputed from two registers per tile instead of being kept in a dozen (the empty asm hides that they do not
+// change): an exclusive-or per read is free next to the matrix instructions, the registers are not.
+struct ImageReader {
+    int k0, v0;
+    __device__ __forceinline__ explicit ImageReader(int lane) {
+        const int c = lane & 31, h = lane >> 5;
+        k0 = c * 256 + ((h ^ swz(c)) << 4);
+        const int i16 = lane & 15, tq = i16 >> 2, tp = i16 & 3;
+        const int ch = 2 * ((lane >> 4) & 1) + (tp >> 1);
+        v0 = (4 * h + tq) * 256 + ((ch ^ ((tq << 2) | h)) << 4) + 8 * (tp & 1);
+    }
+    __device__ __forceinline__ bf16x8_t k(const char* img, int k2, int ks) const {
+        return *(const bf16x8_t*)(img + 32 * k2 * 256 + (k0 ^ (ks << 5)));
+    }
+    __device__ __forceinline__ bf16x8_t v(const char* img, int st, int db) const {
+        // key quads 16 st + 4 h and 16 st + 4 h + 8: swz differs in bit 1 (chunk ^ 2)
+        const char* p = img + st * 4096;
+        const int at = v0 ^ (db << 6);
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CODA_LDS s16x4_t*)(p + at));
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CODA_LDS s16x4_t*)(p + 2048 + (at ^ 32)));
+        const s16x8_t v8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        return __builtin_bit_cast(bf16x8_t, v8);
+    }
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Few rows (RG groups of 32 per tile): the four waves of a workgroup take KEY tiles in turn, each with its own LDS image, maximum, sum and
+// output; they meet once, at the end.  No barrier in the loop.
+constexpr int FEW_TILE = 32;                                    // keys per tile
+constexpr int FEW_WAVE_LDS = 2 * FEW_TILE * 256;                // K and V image: 16 KiB a wave
+
+template <int RG, bool F8, bool G16>
+__global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(AttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int R = 32 * RG;
+    constexpr int NP = F8 ? 4 : 8;                              // 1 KiB pieces of a K (or V) tile
+    __shared__ float ml[4][2][R];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    const int slot = blockIdx.x % a.nslots, kvh = (blockIdx.x / a.nslots) % a.n_kv, split = blockIdx.x / (a.nslots * a.n_kv);
+    TileRows tr;
+    if (!find_tile<R>(a, slot, tr)) return;
+    const Limits lm = load_limits(a, tr.b);
+    const int last = min(tr.r0 + R, tr.rows) - 1;               // last live row of the tile
+    const int end = limit_of(a, lm, fast_div(a.gdiv, last));    // keys that any row of the tile sees
+    const int all = limit_of(a, lm, fast_div(a.gdiv, tr.r0));   // keys that every row of it sees
+    const int nsp = max(1, (end + a.split_len - 1) / a.split_len);
+    if (split >= nsp) return;
+    const int k_lo = split * a.split_len, k_hi = min(end, k_lo + a.split_len);
+    const size_t head_off = (size_t)kvh * a.pg.head_stride_b;
+    const int* table = a.pg.table + (size_t)tr.b * a.pg.ld_table;
+    const char* kbase = a.k + head_off;
+    const char* vbase = a.v + head_off;
+
+    bf16x8_t qf[RG][8];
+    int lim[RG];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+        const int r = min(tr.r0 + rg * 32 + c, tr.rows - 1);
+        const RowAt at = row_at(a, tr, kvh, r);
+        lim[rg] = limit_of(a, lm, at.token - tr.s0);
+        const char* qp = a.q + (size_t)at.token * a.ldq_b + (size_t)at.head * 256 + h * 16;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) qf[rg][ks] = *(const bf16x8_t*)(qp + ks * 32);
+    }
+
+    char* kimg = lds + wave * FEW_WAVE_LDS;
+    char* vimg = kimg + FEW_TILE * 256;
+    f32x16_t o[RG][4];
+    float m_run[RG], l_run[RG];
+    unsigned long long bad[RG];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[rg][db][i] = 0.f;
+        m_run[rg] = -INFINITY;
+        l_run[rg] = 0.f;
+        bad[rg] = 0;
+    }
+
+    u32x4_t kr[NP], vr[NP];
+    TileSource<FEW_TILE, NP, 1, F8, G16> src;
+    src.first = 0;
+    auto fetch = [&] {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const size_t off = src.at(i);
+            kr[i] = *(const u32x4_t*)(kbase + off);
+            vr[i] = *(const u32x4_t*)(vbase + off);
+            if (!G16 && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // bounds the addresses alive at once
+        }
+    };
+    const ImageWriter<F8> img(lane);
+    const ImageReader rd(lane);
+
+    auto tile = [&](int t, bool part, bool dropped, unsigned int ok) {
+        const int key0 = k_lo + t * FEW_TILE;
+        f32x16_t s[RG];
+#pragma unroll
+        for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[rg][i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+            const bf16x8_t kf = rd.k(kimg, 0, ks);
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) s[rg] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[rg][ks], s[rg], 0, 0, 0);
+        }
+#pragma unroll
+        for (int rg = 0; rg < RG; ++rg) {
+            if (part) {                                         // uniform, and kept a branch by the empty asm
+                asm volatile("" ::: "memory");
+                const int left = lim[rg] - key0 - 4 * h;
+                const unsigned int okh = ok >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = (i & 3) + 8 * (i >> 2);
+                    if (j >= left || !((okh >> j) & 1)) s[rg][i] = -INFINITY;
+                }
+            }
+            float mx = s[rg][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[rg][i]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
+            if (__any(mx > m_run[rg] + RESCALE_THR)) {
+                const float m_new = fmaxf(m_run[rg], mx);
+                // a row that has seen no key yet keeps -inf and nothing to scale
+                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[rg] - m_new);
+                l_run[rg] *= alpha;
+                m_run[rg] = m_new;
+#pragma unroll
+                for (int db = 0; db < 4; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[rg][db][i] *= alpha;
+            }
+            const float neg_m = m_run[rg] == -INFINITY ? 0.f : -m_run[rg];
+            float psum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rg][i], a.scale_log2e, neg_m));
+                s[rg][i] = p;
+                psum += p;
+            }
+            l_run[rg] += psum;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            bf16x8_t ph[RG], pl[RG];
+            // weights as a bf16 pair (value and remainder): the second product per fragment hides under the page loads, and
+            // the weights keep 16 significant bits instead of 8
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float p = s[rg][8 * st + j];
+                    ph[rg][j] = (__bf16)p;
+                    pl[rg][j] = (__bf16)(p - (float)ph[rg][j]);
+                }
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+                const bf16x8_t vf = rd.v(vimg, st, db);
+#pragma unroll
+                for (int rg = 0; rg < RG; ++rg) {
+                    o[rg][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, ph[rg], o[rg][db], 0, 0, 0);
+                    o[rg][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pl[rg], o[rg][db], 0, 0, 0);
+                }
+            }
+        }
+        if (dropped) {
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) bad[rg] |= find_nonfinite<F8>(a, table, head_off, key0, FEW_TILE, k_hi, lim[rg], h);
+        }
+    };
+
+    const int nt = (k_hi - k_lo + FEW_TILE - 1) / FEW_TILE;     // may be <= 0: rows that see no key
+    if (wave < nt) {
+        src.look_up(a, table, k_lo + wave * FEW_TILE, k_hi);
+        src.resolve(a, k_lo + wave * FEW_TILE, k_hi);
+        fetch();
+        src.look_up(a, table, k_lo + (wave + 4) * FEW_TILE, k_hi);
+        for (int t = wave; t < nt; t += 4) {
+            const unsigned int ok = (unsigned int)src.ok;
+            const bool part = ok != 0xffffffffu || k_lo + (t + 1) * FEW_TILE > all;      // wave-uniform
+            bool dropped = false;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                if (part) dropped |= img.template put<true>(kimg, vimg, i, kr[i], vr[i], ok);
+                else img.template put<false>(kimg, vimg, i, kr[i], vr[i], ok);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 4 < nt) {
+                src.resolve(a, k_lo + (t + 4) * FEW_TILE, k_hi);
+                fetch();
+                src.look_up(a, table, k_lo + (t + 8) * FEW_TILE, k_hi);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            tile(t, part, __any(dropped), ok);
+        }
+    }
+
+    // ---- the four waves' triples: common maximum, scaled sums
+    float l_half[RG];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+        poison(o[rg], bad[rg]);
+        l_half[rg] = l_run[rg] + __shfl_xor(l_run[rg], 32, 64);
+        if (h == 0) {
+            ml[wave][0][rg * 32 + c] = m_run[rg];
+            ml[wave][1][rg * 32 + c] = l_half[rg];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+        const int r = rg * 32 + c;
+        float m = ml[0][0][r];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][0][r]);
+        // a wave without a maximum holds sums of 0, or NaN where every score it saw was NaN: nothing to scale
+        const float f = m_run[rg] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[rg] - m);
+        // a wave's own image region holds its 32 x 128 fp32 block: 16-byte chunk ch of row r at ch ^ r
+        char* ob = lds + wave * FEW_WAVE_LDS;
+        if (rg > 0) __syncthreads();                            // the block of the previous row group has been read
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                f32x4_t x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = o[rg][db][4 * i4 + j] * f;
+                *(f32x4_t*)(ob + c * 512 + (((8 * db + 2 * i4 + h) ^ c) << 4)) = x;
+            }
+        __syncthreads();
+        // wave w joins rows 8 w .. 8 w + 7: lane -> row, 16 features
+        const int rr = wave * 8 + (lane >> 3), ch0 = (lane & 7) * 4;
+        const int tile_row = tr.r0 + rg * 32 + rr;
+        float acc[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+        float mm = ml[0][0][rg * 32 + rr], ll = 0.f;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, ml[w][0][rg * 32 + rr]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = ml[w][0][rg * 32 + rr];
+            ll += ml[w][1][rg * 32 + rr] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - mm));
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const f32x4_t x = *(const f32x4_t*)(lds + w * FEW_WAVE_LDS + rr * 512 + (((ch0 + q4) ^ rr) << 4));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[4 * q4 + j] += x[j];
+            }
+        }
+        if (tile_row >= tr.rows) continue;
+        const RowAt at = row_at(a, tr, kvh, tile_row);
+        if (nsp == 1) {
+            const float inv = ll == 0.f ? 0.f : a.v_scale / ll;            // no key seen: zeros
+            char* op = a.out + (size_t)at.token * a.ldo_b + (size_t)at.head * 256 + ch0 * 8;
+#pragma unroll
+            for (int q8 = 0; q8 < 2; ++q8) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = acc[8 * q8 + j] * inv;
+                *(u32x4_t*)(op + q8 * 16) = pack8(y);
+            }
+        } else {
+            const size_t row = (size_t)split * a.T * a.n_q + (size_t)at.token * a.n_q + at.head;
+            float* op = a.po + row * HEAD_DIM + ch0 * 4;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) *(f32x4_t*)(op + 4 * q4) = (f32x4_t){acc[4 * q4], acc[4 * q4 + 1], acc[4 * q4 + 2], acc[4 * q4 + 3]};
+            if ((lane & 7) == 0) *(f32x2_t*)(a.pml + row * 2) = (f32x2_t){mm, ll};
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Many rows: NW waves of 32 rows each share a double-buffered stream of 64-key tiles.
+constexpr int MANY_TILE = 64;
+constexpr int MANY_BUF = 2 * MANY_TILE * 256;                   // K and V image: 32 KiB
+
+template <int NW, bool F8, bool G16>
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kernel(AttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int R = 32 * NW;
+    constexpr int NP = (F8 ? 8 : 16) / NW;                      // 1 KiB pieces of a K (or V) tile per wave
+    __shared__ int dropped_s[4];                                // tile t & 3: non-finite values were dropped from its V image
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    // tiles of a sequence read the same keys: consecutive slots of one head run on one XCD and share its L2
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int slot = id % a.nslots, kvh = (id / a.nslots) % a.n_kv, split = id / (a.nslots * a.n_kv);
+    TileRows tr;
+    if (!find_tile<R>(a, slot, tr)) return;
+    const Limits lm = load_limits(a, tr.b);
+    const int last = min(tr.r0 + R, tr.rows) - 1;
+    const int end = limit_of(a, lm, fast_div(a.gdiv, last));
+    const int all = limit_of(a, lm, fast_div(a.gdiv, tr.r0));
+    const int nsp = max(1, (end + a.split_len - 1) / a.split_len);
+    if (split >= nsp) return;
+    const int k_lo = split * a.split_len, k_hi = min(end, k_lo + a.split_len);
+    const size_t head_off = (size_t)kvh * a.pg.head_stride_b;
+    const int* table = a.pg.table + (size_t)tr.b * a.pg.ld_table;
+    const char* kbase = a.k + head_off;
+    const char* vbase = a.v + head_off;
+
+    const int my_row = tr.r0 + wave * 32 + c;
+    const RowAt at = row_at(a, tr, kvh, min(my_row, tr.rows - 1));
+    const int lim = limit_of(a, lm, at.token - tr.s0);
+    // what this wave's rows see: all of them / any of them (limits do not decrease along the rows)
+    const int w_all = __builtin_amdgcn_readlane(lim, 0), w_any = __builtin_amdgcn_readlane(lim, 31);
+    bf16x8_t qf[8];
+    {
+        const char* qp = a.q + (size_t)at.token * a.ldq_b + (size_t)at.head * 256 + h * 16;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) qf[ks] = *(const bf16x8_t*)(qp + ks * 32);
+    }
+    f32x16_t o[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    unsigned long long bad = 0;
+
+    u32x4_t kr[NP], vr[NP];
+    TileSource<MANY_TILE, NP, NW, F8, G16> src;
+    src.first = wave;
+    auto fetch = [&] {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const size_t off = src.at(i);
+            kr[i] = *(const u32x4_t*)(kbase + off);
+            vr[i] = *(const u32x4_t*)(vbase + off);
+        }
+    };
+    const ImageWriter<F8> img(lane);
+    const ImageReader rd(lane);
+
+    auto tile = [&](int t, const char* kimg, bool part, unsigned long long ok) {
+        const char* vimg = kimg + MANY_TILE * 256;
+        f32x16_t s[2];
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[k2][i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) s[k2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rd.k(kimg, k2, ks), qf[ks], s[k2], 0, 0, 0);
+        }
+        if (part) {                                             // uniform, and kept a branch by the empty asm
+            asm volatile("" ::: "memory");
+            const int left = lim - k_lo - t * MANY_TILE - 4 * h;
+            const unsigned long long okh = ok >> (4 * h);
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = 32 * k2 + (i & 3) + 8 * (i >> 2);
+                    if (j >= left || !((okh >> j) & 1)) s[k2][i] = -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[k2][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
+        if (__any(mx > m_run + RESCALE_THR)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            l_run *= alpha;
+            m_run = m_new;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+        }
+        const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+        float psum = 0.f;
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k2][i], a.scale_log2e, neg_m));
+                s[k2][i] = p;
+                psum += p;
+            }
+        l_run += psum;
+        // weights rounded to bf16 for the matrix unit (half a step: 2^-8 of each weight at most); the sum l keeps them in fp32
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+            bf16x8_t pf;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[st >> 1][8 * (st & 1) + j];
+#pragma unroll
+            for (int db = 0; db < 4; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rd.v(vimg, st, db), pf, o[db], 0, 0, 0);
+        }
+    };
+
+    const int nt = (k_hi - k_lo + MANY_TILE - 1) / MANY_TILE;
+    if (threadIdx.x < 4) dropped_s[threadIdx.x] = 0;
+    __syncthreads();
+    if (nt > 0) {
+        auto resolve = [&](int t) { src.resolve(a, k_lo + t * MANY_TILE, k_hi); };
+        auto look_up = [&](int t) { src.look_up(a, table, k_lo + t * MANY_TILE, k_hi); };
+        // registers -> image of tile t; partly seen by the WORKGROUP's rows: it must hold finite values and zeros only
+        auto publish = [&](int t, unsigned long long ok) {
+            char* kimg = lds + (t & 1) * MANY_BUF;
+            char* vimg = kimg + MANY_TILE * 256;
+            if (ok != ~0ull || k_lo + (t + 1) * MANY_TILE > all) {
+                bool dropped = false;
+#pragma unroll
+                for (int i = 0; i < NP; ++i) dropped |= img.template put<true>(kimg, vimg, i * NW + wave, kr[i], vr[i], ok);
+                if (dropped) dropped_s[t & 3] = 1;
+            } else {
+#pragma unroll
+                for (int i = 0; i < NP; ++i) img.template put<false>(kimg, vimg, i * NW + wave, kr[i], vr[i], ok);
+            }
+        };
+        look_up(0);
+        resolve(0);
+        fetch();
+        look_up(1);
+        unsigned long long ok = src.ok, ok_next = 0;
+        publish(0, ok);
+        if (nt > 1) {
+            resolve(1);
+            fetch();
+            ok_next = src.ok;
+            look_up(2);
+        }
+        for (int t = 0; t < nt; ++t) {
+            // one barrier a tile: behind it tile t's image is complete and nobody reads tile t - 1's any more
+            __syncthreads();
+            const bool dropped = dropped_s[t & 3] != 0;
+            if (threadIdx.x == 0) dropped_s[(t + 2) & 3] = 0;   // last read two barriers ago, next written behind the next one
+            unsigned long long ok_after = 0;
+            if (t + 1 < nt) {
+                publish(t + 1, ok_next);
+                __builtin_amdgcn_sched_barrier(0);
+                if (t + 2 < nt) {
+                    resolve(t + 2);
+                    fetch();
+                    ok_after = src.ok;
+                    look_up(t + 3);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const char* kimg = lds + (t & 1) * MANY_BUF;
+            const int key0 = k_lo + t * MANY_TILE;
+            if (key0 < w_any) {                                 // else none of this wave's rows sees the tile
+                tile(t, kimg, ok != ~0ull || key0 + MANY_TILE > w_all, ok);
+                if (dropped) bad |= find_nonfinite<F8>(a, table, head_off, key0, MANY_TILE, k_hi, lim, h);
+            }
+            ok = ok_next;
+            ok_next = ok_after;
+        }
+    }
+
+    poison(o, bad);
+    // ---- epilogue (flash_attn.hip): the halves trade groups so that a lane holds 8 consecutive features
+    const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+    const bool live = my_row < tr.rows;
+    if (nsp == 1) {
+        const float inv = l_tot == 0.f ? 0.f : a.v_scale / l_tot;      // no key seen: zeros
+        char* op = a.out + (size_t)at.token * a.ldo_b + (size_t)at.head * 256;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int gA = 2 * j, gB = 2 * j + 1;
+                const unsigned a0 = pack_bf16x2(o[db][4 * gA] * inv, o[db][4 * gA + 1] * inv);
+                const unsigned a1 = pack_bf16x2(o[db][4 * gA + 2] * inv, o[db][4 * gA + 3] * inv);
+                const unsigned b0 = pack_bf16x2(o[db][4 * gB] * inv, o[db][4 * gB + 1] * inv);
+                const unsigned b1 = pack_bf16x2(o[db][4 * gB + 2] * inv, o[db][4 * gB + 3] * inv);
+                const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+                const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+                if (live) *(u32x4_t*)(op + (32 * db + 8 * (2 * j + h)) * 2) = (u32x4_t){s0[0], s1[0], s0[1], s1[1]};
+            }
+    } else if (live) {
+        const size_t row = (size_t)split * a.T * a.n_q + (size_t)at.token * a.n_q + at.head;
+        float* op = a.po + row * HEAD_DIM;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)
+                *(f32x4_t*)(op + 32 * db + 8 * i4 + 4 * h) = (f32x4_t){o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]};
+        if (h == 0) *(f32x2_t*)(a.pml + row * 2) = (f32x2_t){m_run, l_tot};
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Joins the ranges of one (token, head) row: 32 lanes hold its 128 features, the 8 half-waves of the workgroup take ranges in
+// turn and meet in LDS.  R: rows per tile of the kernel that wrote the ranges (a tile's rows have the same number of ranges).
+template <int R>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
+    __shared__ float sm[8], sl[8];
+    __shared__ f32x4_t so[8][32];
+    const int token = blockIdx.x / a.n_q, head = blockIdx.x % a.n_q;
+    const int b = wave_search(a.B, token, [&](int i) { return (long long)clamp_start(a.seq_start, i, a.T); });
+    if (b < 0) return;
+    const int s0 = clamp_start(a.seq_start, b, a.T), n = clamp_start(a.seq_start, b + 1, a.T) - s0;
+    if (token - s0 >= n) return;                                // a row of no sequence
+    const int r = (token - s0) * a.g + head % a.g;
+    const int last = (int)min(((long long)r / R + 1) * R, (long long)n * a.g) - 1;
+    const Limits lm = load_limits(a, b);
+    const int end = limit_of(a, lm, fast_div(a.gdiv, last));
+    const int nsp = (end + a.split_len - 1) / a.split_len;
+    if (nsp <= 1) return;                                       // written by the first kernel
+    const int grp = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const size_t rows = (size_t)a.T * a.n_q, row = (size_t)blockIdx.x;
+    float m = -INFINITY, sum = 0.f;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = grp; s < nsp; s += 8) {
+        const f32x2_t e = *(const f32x2_t*)(a.pml + (s * rows + row) * 2);
+        const f32x4_t x = *(const f32x4_t*)(a.po + (s * rows + row) * HEAD_DIM + 4 * l);
+        const float mn = fmaxf(m, e[0]);                        // -inf: no key of the range was seen, sums of 0
+        const float fo = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float fn = e[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(e[0] - mn);
+        sum = sum * fo + e[1] * fn;
+        acc = acc * fo + x * fn;
+        m = mn;
+    }
+    if (l == 0) { sm[grp] = m; sl[grp] = sum; }
+    so[grp][l] = acc;
+    __syncthreads();
+    if (grp) return;
+    float mm = sm[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mm = fmaxf(mm, sm[i]);
+    float tot = 0.f;
+    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = sm[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[i] - mm);
+        tot += sl[i] * f;
+        y = y + so[i][l] * f;
+    }
+    const float inv = tot == 0.f ? 0.f : a.v_scale / tot;
+    *(u32x2_t*)(a.out + (size_t)token * a.ldo_b + (size_t)head * 256 + l * 8) =
+        (u32x2_t){pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
+}
+
+// How a call is cut: rows per tile, tile slots, key ranges.  A function of the call's sizes alone.
+struct Plan {
+    int R; long long nslots; int nsplit, split_len;
+};
+
+Plan make_plan(int T, int B, int max_kv, int n_q, int n_kv, int cus) {
+    const int g = n_q / n_kv;
+    const double rho = (double)T * g / B;                       // rows per sequence and key/value head, on average
+    Plan p;
+    p.R = rho <= 32 ? 32 : rho <= 64 ? 64 : rho <= 128 ? 128 : 256;
+    p.nslots = (long long)T * g / p.R + B;
+    // ranges: enough workgroups for two per CU (one where a workgroup has the CU to itself), none shorter than 256 keys
+    const long long tiles = (((long long)T * g + p.R - 1) / p.R > B ? ((long long)T * g + p.R - 1) / p.R : B) * n_kv;
+    const long long want = (p.R == 32 || p.R == 128 ? 2 : 1) * (long long)cus;
+    long long ns = (want + tiles - 1) / tiles;
+    const long long most = (max_kv + 255) / 256;
+    if (ns > most) ns = most;
+    if (ns > MAX_SPLITS) ns = MAX_SPLITS;
+    if (ns < 1) ns = 1;
+    p.split_len = max_kv > 0 ? (int)((max_kv + ns - 1) / ns) : 1;
+    p.split_len = (p.split_len + 127) / 128 * 128;
+    p.nsplit = max_kv > 0 ? (max_kv + p.split_len - 1) / p.split_len : 1;
+    return p;
+}
+
+long long plan_bytes(const Plan& p, int T, int n_q) { return p.nsplit > 1 ? (long long)p.nsplit * T * n_q * (HEAD_DIM + 2) * 4 : 0; }
+
+}  // namespace
+
+extern "C" long long coda_paged_attn_workspace_bytes(int T, int B, int max_kv, int n_q, int n_kv) {
+    if (T <= 0 || B <= 0 || max_kv < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv) return 0;
+    return plan_bytes(make_plan(T, B, max_kv, n_q, n_kv, coda_device_cus()), T, n_q);
+}
+
+extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long long ld_out, const int* seq_start, const int* pos0,
+                               const int* kv_len, int B, int T, const int* page_table, long long ld_table, int max_pages,
+                               const void* k_cache, const void* v_cache, long long page_stride, int num_pages, int page_size,
+                               int cache_type, float k_scale, float v_scale, int max_kv, int n_q, int n_kv, float scale, int mask_block,
+                               void* workspace, long long workspace_bytes, void* stream) {
+    const char* who = "coda_paged_attn";
+    if (B <= 0 || T <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv) return coda_refuse(who, CODA_ERR_SHAPE, "a size is not positive, or n_q % n_kv");
+    if ((long long)T * n_q > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "T * n_q exceeds 2^31 - 1");
+    if (max_kv < 0 || (long long)max_kv > (long long)max_pages * page_size) return coda_refuse(who, CODA_ERR_SHAPE, "max_kv is not within max_pages * page_size");
+    if (ld_q < (long long)n_q * HEAD_DIM || ld_out < (long long)n_q * HEAD_DIM) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");
+    if (!q || !out || !seq_start || !pos0 || !kv_len) return coda_refuse(who, CODA_ERR_ARG, "null pointer");
+    if (!(scale > 0.f) || scale > 1e30f) return coda_refuse(who, CODA_ERR_ARG, "scale must be positive and finite");
+    if (mask_block < 0) return coda_refuse(who, CODA_ERR_ARG, "mask_block is negative");
+    if (((uintptr_t)q | (uintptr_t)out) & 15 || (ld_q * 2) % 16 || (ld_out * 2) % 16) return coda_refuse(who, CODA_ERR_ALIGN, "rows start on 16 bytes");
+    AttnArgs a;
+    const int rc = coda_check_pages(who, k_cache, v_cache, page_table, ld_table, max_pages, page_stride, num_pages, page_size, cache_type,
+                                    k_scale, v_scale, n_kv, &a.pg);
+    if (rc != CODA_OK) return rc;
+    const Plan p = make_plan(T, B, max_kv, n_q, n_kv, coda_device_cus());
+    const long long need = plan_bytes(p, T, n_q);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_paged_attn_workspace_bytes");
+    if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
+    const long long wgs = p.nslots * n_kv * p.nsplit;
+    if (wgs > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
+    const bool f8 = cache_type == CODA_CACHE_E4M3;
+    a.q = (const char*)q; a.ldq_b = ld_q * 2;
+    a.out = (char*)out; a.ldo_b = ld_out * 2;
+    a.seq_start = seq_start; a.pos0 = pos0; a.kv_len = kv_len;
+    a.B = B; a.T = T; a.max_kv = max_kv;
+    a.k = (const char*)k_cache; a.v = (const char*)v_cache;
+    a.n_q = n_q; a.n_kv = n_kv; a.g = n_q / n_kv; a.gdiv = make_fast_div((unsigned)a.g);
+    a.mask_block = mask_block;
+    a.scale_log2e = scale * (f8 ? k_scale : 1.0f) * 1.4426950408889634f;
+    a.v_scale = f8 ? v_scale : 1.0f;
+    a.nslots = (int)p.nslots; a.nsplit = p.nsplit; a.split_len = p.split_len;
+    a.po = (float*)workspace;
+    a.pml = p.nsplit > 1 ? (float*)workspace + (long long)p.nsplit * T * n_q * HEAD_DIM : nullptr;
+    hipStream_t st = (hipStream_t)stream;
+    auto go = [&](auto kernel, int threads, int lds) -> int {
+        if (coda_ensure_dyn_lds((const void*)kernel, lds) != CODA_OK) return CODA_ERR_LAUNCH;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(threads), lds, st, a);
+        CODA_CHECK_LAUNCH("paged_attn");
+        return CODA_OK;
+    };
+    // pages of a multiple of 16 keys take the kernels that address 16 keys at a time
+    auto pick = [&](auto f8c, auto g16c) -> int {
+        constexpr bool F8 = decltype(f8c)::value, G16 = decltype(g16c)::value;
+        if (p.R == 32) return go(paged_attn_few_kernel<1, F8, G16>, 256, 4 * FEW_WAVE_LDS);
+        if (p.R == 64) return go(paged_attn_few_kernel<2, F8, G16>, 256, 4 * FEW_WAVE_LDS);
+        if (p.R == 128) return go(paged_attn_many_kernel<4, F8, G16>, 256, 2 * MANY_BUF);
+        return go(paged_attn_many_kernel<8, F8, G16>, 512, 2 * MANY_BUF);
+    };
+    const bool g16 = page_size % 16 == 0;
+    const std::true_type yes{};
+    const std::false_type no{};
+    const int r2 = f8 ? (g16 ? pick(yes, yes) : pick(yes, no)) : (g16 ? pick(no, yes) : pick(no, no));
+    if (r2 != CODA_OK || p.nsplit == 1) return r2;
+    const dim3 jg((unsigned)((long long)T * n_q));
+    if (p.R == 32) hipLaunchKernelGGL(paged_attn_join_kernel<32>, jg, dim3(256), 0, st, a);
+    else if (p.R == 64) hipLaunchKernelGGL(paged_attn_join_kernel<64>, jg, dim3(256), 0, st, a);
+    else if (p.R == 128) hipLaunchKernelGGL(paged_attn_join_kernel<128>, jg, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(paged_attn_join_kernel<256>, jg, dim3(256), 0, st, a);
+    CODA_CHECK_LAUNCH("paged_attn join");
+    return CODA_OK;
+}

@@ -236,6 +236,55 @@ int coda_select_threshold(long long* x, const float* conf, const long long* x0, 
 int coda_origin_transfer(long long* x, const long long* x0, const int* dst_pos, const int* count, int max_rows,
                          const float* u, unsigned long long seed, float p_transfer, void* stream);
 
+/* ---- ragged batches over a paged key/value cache ---------------------------------------------------------------------
+ * NO COUNTERPART IN THE REFERENCE (which recomputes every sequence and keeps no cache): for serving many requests of
+ * different lengths, or one denoise block behind a prefix that is kept.
+ *
+ * Batch.  T packed token rows; sequence b < B owns rows seq_start[b] .. seq_start[b+1]-1 (seq_start int32 [B+1] on the
+ * device, not decreasing, within [0, T]; a sequence may have no row).  Rows of no sequence are neither read nor written.
+ * Cache.  k_cache / v_cache: pages [num_pages][n_kv][page_size][128], page_stride ELEMENTS from page to page (at least
+ * n_kv * page_size * 128), both of the same geometry; page_size is any positive number.  Position p of sequence b lives in slot
+ * p % page_size of page page_table[b * ld_table + p / page_size] (int32 on the device, max_pages entries a sequence).  An
+ * entry outside [0, num_pages) is a page that is not there: nothing is stored to it and its keys are not seen.
+ * cache_type: CODA_CACHE_BF16, or CODA_CACHE_E4M3 (OCP e4m3, value = k_scale / v_scale * stored, scales in [1e-30, 1e30];
+ * ignored for bf16).  head_dim is 128. */
+#define CODA_CACHE_BF16 0
+#define CODA_CACHE_E4M3 1
+#define CODA_APPEND_STEPWISE 1 /* round to bf16 after every operation: the bits of coda_qknorm_rope */
+
+/* q_norm / k_norm + rotary embedding (the arithmetic of coda_qknorm_rope) of new tokens, q to q_out, k and v into the cache.
+ * qkv bf16 [T, (n_q + 2 n_kv) * 128]: q heads, then k heads, then v heads.  Token i of sequence b has position pos0[b] + i
+ * (pos0 int32 [B]), which picks its row of cos / sin (bf16 [max_pos, 128]) and its slot.  q_weight / k_weight bf16 [128], or
+ * both NULL: no norm.  q_out bf16 [T, n_q * 128]: the q columns of qkv (in place) or memory apart from qkv.
+ * Arithmetic in fp32, rounded once to the stored type (e4m3: times the fp32 reciprocal of the scale, to nearest even,
+ * clamped to +-448); flags CODA_APPEND_STEPWISE: bf16 rounding after every operation as coda_qknorm_rope does, so that a cached
+ * key has the bits that the uncached forward computes.  A token whose position is outside [0, max_pos) is skipped whole;
+ * one whose page is not there gets its q row only.  Two tokens of one call must not share a slot (which one stays, or which
+ * part of either, is not defined). */
+int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out, long long ld_q, const void* q_weight,
+                      const void* k_weight, const void* cos, const void* sin, int max_pos, const int* seq_start,
+                      const int* pos0, int B, int T, const int* page_table, long long ld_table, int max_pages, void* k_cache,
+                      void* v_cache, long long page_stride, int num_pages, int page_size, int cache_type, float k_scale,
+                      float v_scale, int n_q, int n_kv, float eps, int flags, void* stream);
+
+/* Attention of the new tokens' queries over the cache: out_i = softmax_j(scale q_i . K_j) V, n_q % n_kv == 0, from one token a
+ * sequence (decode) to whole prompts.  q and out bf16 [T, n_q * 128] (out apart from q and the cache).  Sequence b has
+ * kv_len[b] keys, positions 0 .. kv_len[b]-1 (int32 [B]).  mask_block 0: a token sees all of them, later positions included
+ * (the denoiser's attention).  mask_block m > 0: token i sees the keys before the end of its block of m positions,
+ * j < ((pos0[b] + i) / m + 1) * m (1: causal).  A token that sees no key gets zeros.  Keys a token does not see
+ * have no influence on it, whatever their slots hold; an infinity or NaN that it does see makes its output non-finite.
+ * max_kv: host-side bound of kv_len, at most max_pages * page_size (keys from max_kv on are not seen): it sizes the launch.
+ * Scores, maxima, sums and outputs are fp32; weights enter the second product as bf16 (a bf16 pair where there are at most 64
+ * rows per sequence and key/value head).  scale > 0.
+ * workspace: coda_paged_attn_workspace_bytes(T, B, max_kv, n_q, n_kv) bytes (may be 0), 16-byte aligned, contents irrelevant before
+ * and after; calls that may run at the same time need one each. */
+long long coda_paged_attn_workspace_bytes(int T, int B, int max_kv, int n_q, int n_kv);
+int coda_paged_attn(const void* q, long long ld_q, void* out, long long ld_out, const int* seq_start, const int* pos0,
+                    const int* kv_len, int B, int T, const int* page_table, long long ld_table, int max_pages,
+                    const void* k_cache, const void* v_cache, long long page_stride, int num_pages, int page_size,
+                    int cache_type, float k_scale, float v_scale, int max_kv, int n_q, int n_kv, float scale, int mask_block,
+                    void* workspace, long long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,89 @@
+"""Argument checks of the ragged-batch entry points (paged cache, low-rank adapters): every refusal returns its code and
+words before anything is launched, so none of this needs a GPU - and none of these calls may reach one."""
+import os
+
+import pytest
+
+from coda_amd import _lib
+
+P = 1 << 20          # stands for an aligned device pointer: a refused call never follows it
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built():
+    if not os.path.exists(_lib.LIB_PATH):
+        import __graft_entry__
+        __graft_entry__.build()
+
+
+APPEND = dict(qkv=P, ld_qkv=32 * 128, q_out=P, ld_q=16 * 128, q_weight=P, k_weight=P, cos=P, sin=P, max_pos=64, seq_start=P, pos0=P, B=2,
+              T=4, page_table=P, ld_table=8, max_pages=8, k_cache=P, v_cache=P, page_stride=8 * 16 * 128, num_pages=16, page_size=16,
+              cache_type=0, k_scale=1.0, v_scale=1.0, n_q=16, n_kv=8, eps=1e-6, flags=0, stream=None)
+ATTN = dict(q=P, ld_q=16 * 128, out=P, ld_out=16 * 128, seq_start=P, pos0=P, kv_len=P, B=2, T=4, page_table=P, ld_table=8, max_pages=8,
+            k_cache=P, v_cache=P, page_stride=8 * 16 * 128, num_pages=16, page_size=16, cache_type=0, k_scale=1.0, v_scale=1.0,
+            max_kv=128, n_q=16, n_kv=8, scale=0.1, mask_block=0, workspace=P, workspace_bytes=1 << 30, stream=None)
+
+NAN, INF = float("nan"), float("inf")
+PAGES = [  # the checks of a cache are the same for both entry points
+    (dict(k_cache=None), "ARG", "null cache"), (dict(v_cache=None), "ARG", "null cache"), (dict(page_table=None), "ARG", "null cache"),
+    (dict(cache_type=2), "ARG", "cache type"), (dict(cache_type=-1), "ARG", "cache type"),
+    (dict(cache_type=1, k_scale=0.0), "ARG", "scales"), (dict(cache_type=1, v_scale=-1.0), "ARG", "scales"),
+    (dict(cache_type=1, v_scale=NAN), "ARG", "scales"), (dict(cache_type=1, k_scale=INF), "ARG", "scales"),
+    (dict(cache_type=1, k_scale=1e-38), "ARG", "scales"),
+    (dict(num_pages=0), "SHAPE", "page table"), (dict(page_size=0), "SHAPE", ""), (dict(page_size=-16), "SHAPE", ""),
+    (dict(ld_table=7), "SHAPE", "page table"), (dict(max_pages=1 << 28, ld_table=1 << 28), "SHAPE", "2^31"),
+    (dict(page_stride=8 * 16 * 128 - 8), "SHAPE", "page_stride"), (dict(page_stride=8 * 16 * 128 + 4), "ALIGN", "16 bytes"),
+    (dict(k_cache=P + 8), "ALIGN", "16 bytes"), (dict(v_cache=P + 2), "ALIGN", "16 bytes"),
+    (dict(cache_type=1, page_stride=8 * 16 * 128 + 8), "ALIGN", "16 bytes"),
+]
+BATCH = [(dict(B=0), "SHAPE", ""), (dict(B=-1), "SHAPE", ""), (dict(T=0), "SHAPE", ""), (dict(n_q=0), "SHAPE", ""), (dict(n_kv=0), "SHAPE", ""),
+         (dict(seq_start=None), "ARG", "null"), (dict(pos0=None), "ARG", "null")]
+
+
+def refused(name, base, change, code, words):
+    args = {**base, **change}
+    with pytest.raises(_lib.CodaHipError) as e:
+        _lib.call(name, *args.values())
+    assert f"CODA_ERR_{code}" in str(e.value), str(e.value)
+    assert words in str(e.value)
+    # worded, and by its own name: a stale message of another call would not be shown
+    assert f" {name}: " in str(e.value), str(e.value)
+
+
+@pytest.mark.parametrize("change,code,words", PAGES + BATCH + [
+    (dict(max_pos=0), "SHAPE", ""), (dict(ld_qkv=32 * 128 - 8), "SHAPE", "stride"), (dict(ld_q=16 * 128 - 8), "SHAPE", "stride"),
+    (dict(qkv=None), "ARG", "null"), (dict(q_out=None), "ARG", "null"), (dict(cos=None), "ARG", "null"), (dict(sin=None), "ARG", "null"),
+    (dict(q_weight=None), "ARG", "together"), (dict(k_weight=None), "ARG", "together"), (dict(flags=2), "ARG", "flag"),
+    (dict(qkv=P + 2), "ALIGN", "16 bytes"), (dict(cos=P + 8), "ALIGN", "16 bytes"), (dict(k_weight=P + 4), "ALIGN", "16 bytes"),
+    (dict(ld_qkv=32 * 128 + 4), "ALIGN", "16 bytes"), (dict(ld_q=16 * 128 + 2), "ALIGN", "16 bytes"),
+    (dict(n_q=2000000, ld_qkv=1 << 40), "SHAPE", "heads"),
+])
+def test_append_refuses(change, code, words):
+    refused("coda_paged_append", APPEND, change, code, words)
+
+
+@pytest.mark.parametrize("change,code,words", PAGES + BATCH + [
+    (dict(kv_len=None), "ARG", "null"), (dict(q=None), "ARG", "null"), (dict(out=None), "ARG", "null"),
+    (dict(n_q=15), "SHAPE", "n_q"), (dict(max_kv=129), "SHAPE", "max_kv"), (dict(max_kv=-1), "SHAPE", "max_kv"),
+    (dict(max_pages=0), "SHAPE", ""), (dict(ld_q=16 * 128 - 8), "SHAPE", "stride"), (dict(ld_out=16 * 128 - 8), "SHAPE", "stride"),
+    (dict(scale=0.0), "ARG", "scale"), (dict(scale=-0.1), "ARG", "scale"), (dict(scale=NAN), "ARG", "scale"), (dict(scale=INF), "ARG", "scale"),
+    (dict(mask_block=-1), "ARG", "mask_block"), (dict(q=P + 8), "ALIGN", ""), (dict(ld_out=16 * 128 + 4), "ALIGN", ""),
+    (dict(T=1 << 28), "SHAPE", "2^31"),
+    # 4096 keys are more than one range: the workspace has to be there
+    (dict(max_kv=4096, max_pages=256, ld_table=256, workspace_bytes=1024), "ARG", "workspace"),
+    (dict(max_kv=4096, max_pages=256, ld_table=256, workspace=None), "ARG", "workspace"),
+    (dict(max_kv=4096, max_pages=256, ld_table=256, workspace=P + 4), "ALIGN", "workspace"),
+])
+def test_attn_refuses(change, code, words):
+    refused("coda_paged_attn", ATTN, change, code, words)
+
+
+def test_attn_workspace_sizes():
+    size = _lib.load().coda_paged_attn_workspace_bytes
+    assert size(1, 1, 0, 16, 8) == 0 and size(1, 1, 256, 16, 8) == 0          # one range of keys: joined by nobody
+    assert size(1, 1, 4096, 16, 8) > 0
+    assert size(0, 1, 4096, 16, 8) == 0 and size(1, 1, 4096, 16, 7) == 0      # sizes that the call itself refuses
+    for T, B, kv in ((1, 1, 40960), (4, 4, 40960), (128, 128, 2048), (8192, 8, 4096)):
+        # a partial output and two numbers per range, token and head; never more ranges than 256 keys each would give
+        assert size(T, B, kv, 16, 8) % (T * 16 * 130 * 4) == 0
+        assert size(T, B, kv, 16, 8) <= -(-kv // 256) * T * 16 * 130 * 4
