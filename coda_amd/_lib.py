@@ -50,6 +50,8 @@ SIGNATURES = {
     "coda_paged_attn_workspace_bytes": (_ll, [_i, _i, _i, _i, _i]),
     "coda_paged_attn": (_i, [_p, _ll, _p, _ll, _p, _p, _p, _i, _i, _p, _ll, _i, _p, _p, _ll, _i, _i, _i, _f, _f, _i, _i, _i, _f, _i, _p,
                              _ll, _p]),
+    "coda_lora_workspace_bytes": (_ll, [_i, _i, _i, _i, _i]),
+    "coda_lora_bf16": (_i, [_p, _ll, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _ll, _p, _ll, _i, _i, _p, _ll, _p]),
     "coda_origin_transfer": (_i, [_p, _p, _p, _p, _i, _p, _ull, _f, _p]),
 }
 

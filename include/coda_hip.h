@@ -285,6 +285,20 @@ int coda_paged_attn(const void* q, long long ld_q, void* out, long long ld_out, 
                     int cache_type, float k_scale, float v_scale, int max_kv, int n_q, int n_kv, float scale, int mask_block,
                     void* workspace, long long workspace_bytes, void* stream);
 
+/* Low-rank adapters of many requests beside a shared projection, on the ragged batch above:
+ *   C[t] = R[t] + scale[a] (X[t] A[a]^T) B[a]^T,   a = adapter[b] of the sequence b that owns row t.
+ * X bf16 [T, K] (the projection's input), R bf16 [T, N] (its output, e.g. of coda_gemm_bf16 CODA_EPI_PLAIN), C bf16 [T, N]: R
+ * itself (in place) or memory apart from R and X.  A bf16 [n_adapters, rank, K], B bf16 [n_adapters, N, rank], both dense; scale
+ * fp32 [n_adapters] on the device or NULL (1); adapter int32 [B], a value outside [0, n_adapters) means none: C[t] = R[t].
+ * rank is a multiple of 8 up to 128 (adapters of smaller rank: zero rows of A), K % 64 == 0, N % 8 == 0.  Both products are summed in
+ * fp32 and the result is rounded once; X A^T enters the second one as a bf16 pair (16 significant bits).
+ * workspace: coda_lora_workspace_bytes(T, B, N, K, rank) bytes, 16-byte aligned, contents irrelevant before and after; calls
+ * that may run at the same time need one each. */
+long long coda_lora_workspace_bytes(int T, int B, int N, int K, int rank);
+int coda_lora_bf16(const void* X, long long ldx, const void* A, const void* Bw, const float* scale, const int* seq_start,
+                   const int* adapter, int B, int T, int n_adapters, int rank, const void* R, long long ldr, void* C,
+                   long long ldc, int N, int K, void* workspace, long long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -87,3 +87,29 @@ def test_attn_workspace_sizes():
         # a partial output and two numbers per range, token and head; never more ranges than 256 keys each would give
         assert size(T, B, kv, 16, 8) % (T * 16 * 130 * 4) == 0
         assert size(T, B, kv, 16, 8) <= -(-kv // 256) * T * 16 * 130 * 4
+
+
+LORA = dict(X=P, ldx=256, A=P, Bw=P, scale=None, seq_start=P, adapter=P, B=2, T=4, n_adapters=3, rank=16, R=P, ldr=512, C=P, ldc=512, N=512,
+            K=256, workspace=P, workspace_bytes=1 << 30, stream=None)
+
+
+@pytest.mark.parametrize("change,code,words", [
+    (dict(B=0), "SHAPE", "positive"), (dict(T=0), "SHAPE", "positive"), (dict(T=-3), "SHAPE", "positive"), (dict(n_adapters=0), "SHAPE", "positive"),
+    (dict(N=0), "SHAPE", "positive"), (dict(K=0), "SHAPE", "positive"), (dict(rank=0), "SHAPE", "rank"), (dict(rank=12), "SHAPE", "rank"),
+    (dict(rank=136), "SHAPE", "rank"), (dict(K=224), "SHAPE", "K % 64"), (dict(N=508), "SHAPE", "N % 8"), (dict(ldx=248), "SHAPE", "stride"),
+    (dict(ldr=504), "SHAPE", "stride"), (dict(ldc=504), "SHAPE", "stride"),
+    *[(dict([(n, None)]), "ARG", "null") for n in ("X", "A", "Bw", "seq_start", "adapter", "R", "C")],
+    *[(dict([(n, P + 8)]), "ALIGN", "16 bytes") for n in ("X", "A", "Bw", "R", "C")],
+    (dict(ldx=260), "ALIGN", "16 bytes"), (dict(ldr=516), "ALIGN", "16 bytes"), (dict(ldc=516), "ALIGN", "16 bytes"),
+    (dict(workspace=None), "ARG", "workspace"), (dict(workspace_bytes=64), "ARG", "workspace"), (dict(workspace=P + 8), "ALIGN", "workspace"),
+])
+def test_lora_refuses(change, code, words):
+    refused("coda_lora_bf16", LORA, change, code, words)
+
+
+def test_lora_workspace_sizes():
+    size = _lib.load().coda_lora_workspace_bytes
+    assert size(0, 1, 512, 256, 16) == 0 and size(4, 2, 512, 256, 0) == 0
+    for T, B, K, rank in ((1, 1, 2048, 16), (32, 32, 2048, 16), (1024, 32, 6144, 64), (16384, 32, 2048, 128)):
+        assert size(T, B, 2048, K, rank) > 0 and size(T, B, 2048, K, rank) % (T * rank * 4) == 0
+        assert size(T, B, 2048, K, rank) <= K // 256 * T * rank * 4
