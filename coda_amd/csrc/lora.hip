@@ -7,10 +7,12 @@
 // adds U B^T to R with R as the start value of the accumulators, so that the result is rounded once.
 //
 // v_mfma_f32_16x16x32_bf16 in both, weights as the A operand: a lane then holds four consecutive outputs (ranks, features) of one
-// token.  Both products read each weight and activation once per tile straight into fragments, 64 B of a row a quarter-wave: there is
-// too little reuse at serving ranks (8 .. 128) for a detour through LDS to pay.  U enters the second product as a bf16 pair
-// (value and remainder): the extra matrix instructions are free in a kernel that waits for memory, and U keeps 16 bits.
+// token.  Both are bound by memory at serving ranks (8 .. 128).  X, A, R and C move as contiguous 512 bytes of a row, through LDS:
+// fragments straight from memory (16 rows x 64 B an instruction) took 27 + 120 us where this takes 22 + 95 (15.5 k tokens, rank 32,
+// 2048 -> 6144).  U enters the second product as a bf16 pair (value and remainder): the extra matrix instructions are free in a
+// kernel that waits for memory, and U keeps 16 bits.
 #include "paged_common.h"
+#include <type_traits>
 
 using namespace paged;
 
@@ -33,84 +35,93 @@ struct Tile {
     int b, s0, n, t0, adapter;                  // sequence, its first row, its tokens; the tile's first token; -1: no adapter
 };
 
-// tile slots of sequence b start at floor(start_b / TM) + b (paged_attn.hip numbers its tiles the same way)
 template <int TM>
 __device__ __forceinline__ bool find_tile(const LoraArgs& a, int slot, Tile& t) {
-    auto first = [&](int i) { return (long long)(clamp_start(a.seq_start, i, a.T) / TM + i); };
-    t.b = wave_search(a.B, slot, first);
-    if (t.b < 0) return false;
-    t.s0 = clamp_start(a.seq_start, t.b, a.T);
-    t.n = clamp_start(a.seq_start, t.b + 1, a.T) - t.s0;
-    const long long t0 = (slot - first(t.b)) * TM;
-    t.t0 = (int)t0;
-    const int ad = a.adapter[t.b];
-    t.adapter = (unsigned)ad < (unsigned)a.n_adapters ? ad : -1;
-    return t0 < t.n;
+    const SeqArrays arr = {a.seq_start, a.adapter, nullptr, a.B, a.T};
+    SeqBlock blk;
+    blk.load(arr, 0);
+    int k;
+    const Seq q = seq_of_item(arr, blk, slot, k, [](const SeqLane& l) { return tiles_of<TM>(l, 1); });
+    if (q.b < 0) return false;
+    t = {q.b, q.s0, q.n, k * TM, (unsigned)q.x < (unsigned)a.n_adapters ? q.x : -1};
+    return true;
 }
 
-// U of 16 MT tokens, 16 RT ranks (those beyond the adapter's are computed from its last row and dropped)
+// U of 16 MT tokens, 16 RT ranks (those beyond the adapter's are computed from its last row and dropped).
+// Steps of 256 elements: rows of X and A come in as contiguous 512 bytes through registers (the next step's fly under this one's
+// products) into an LDS image, 16-byte chunk ch of row r at ch ^ (r & 15), and the four waves take 64 elements of each step.
+template <int MT, int RT>
+struct Down {
+    static constexpr int ROWS = 16 * (MT + RT);
+    static constexpr int NL = ROWS / 8;                         // 16-byte loads per thread and step (8 rows per pass of 256 threads)
+    static constexpr int LDS = ROWS * 512 > 4 * MT * RT * 1024 ? ROWS * 512 : 4 * MT * RT * 1024;
+};
+
 template <int MT, int RT>
 __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
-    __shared__ f32x4_t part[4][MT * RT][64];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int NL = Down<MT, RT>::NL;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = blockIdx.x / a.ksplit, ks = blockIdx.x % a.ksplit;
     Tile t;
     if (!find_tile<16 * MT>(a, slot, t) || t.adapter < 0) return;
-    const int row = lane & 15, quad = lane >> 4;
-    const char* xp[MT];
-    const char* ap[RT];
+    const int lr = threadIdx.x >> 5, lc = threadIdx.x & 31;     // this thread's row (of 8) and chunk in a pass
+    const char* src[NL];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) xp[m] = a.x + (size_t)(t.s0 + min(t.t0 + 16 * m + row, t.n - 1)) * a.ldx_b + quad * 16;
+    for (int i = 0; i < NL; ++i) {
+        const int r = 8 * i + lr;
+        src[i] = (i < 2 * MT ? a.x + (size_t)(t.s0 + min(t.t0 + r, t.n - 1)) * a.ldx_b
+                             : a.a + ((size_t)t.adapter * a.rank + min(r - 16 * MT, a.rank - 1)) * a.K * 2);
+    }
+    const int k0 = ks * a.kchunk, k1 = min(a.K, k0 + a.kchunk);
+    u32x4_t v[NL];
+    auto fetch = [&](int k) {
+        const size_t at = (size_t)min(k + 8 * lc, a.K - 8) * 2; // past K: something that exists; the products stop at k1
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
-        ap[r] = a.a + ((size_t)t.adapter * a.rank + min(16 * r + row, a.rank - 1)) * a.K * 2 + quad * 16;
+        for (int i = 0; i < NL; ++i) v[i] = *(const u32x4_t*)(src[i] + at);
+    };
     f32x4_t acc[MT][RT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[m][r] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    const int k1 = min(a.K, (ks + 1) * a.kchunk);
-    // 64 elements (one 128-byte line of every row) a step, the four waves in turn; the next step's fragments fly under this one's
-    bf16x8_t xf[2][MT], af[2][RT];
-    auto load = [&](int k) {
+    const int row = lane & 15, quad = lane >> 4;
+    fetch(k0);
+    for (int k = k0; k < k1; k += 256) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int i = 0; i < NL; ++i) *(u32x4_t*)(lds + (8 * i + lr) * 512 + ((lc ^ ((8 * i + lr) & 15)) << 4)) = v[i];
+        __syncthreads();
+        if (k + 256 < k1) fetch(k + 256);
+        if (k + 64 * wave < k1) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) xf[s][m] = *(const bf16x8_t*)(xp[m] + (size_t)k * 2 + s * 64);
+            for (int s = 0; s < 2; ++s) {
+                const int at = row * 512 + (((8 * wave + 4 * s + quad) ^ row) << 4);
+                bf16x8_t xf[MT], af[RT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) af[s][r] = *(const bf16x8_t*)(ap[r] + (size_t)k * 2 + s * 64);
+                for (int m = 0; m < MT; ++m) xf[m] = *(const bf16x8_t*)(lds + m * 8192 + at);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) af[r] = *(const bf16x8_t*)(lds + (MT + r) * 8192 + at);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[r], xf[m], acc[m][r], 0, 0, 0);
+            }
         }
-    };
-    int k = ks * a.kchunk + 64 * wave;
-    if (k < k1) load(k);
-    for (; k < k1; k += 256) {
-        bf16x8_t xc[2][MT], ac[2][RT];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m) xc[s][m] = xf[s][m];
-#pragma unroll
-            for (int r = 0; r < RT; ++r) ac[s][r] = af[s][r];
-        }
-        load(min(k + 256, a.K - 64));          // past the range: a line that exists, not used
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int r = 0; r < RT; ++r) acc[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ac[s][r], xc[s][m], acc[m][r], 0, 0, 0);
+        __syncthreads();
     }
+    f32x4_t* part = (f32x4_t*)lds;                              // [4][MT RT][64]
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) part[wave][m * RT + r][lane] = acc[m][r];
+        for (int r = 0; r < RT; ++r) part[(wave * MT * RT + m * RT + r) * 64 + lane] = acc[m][r];
     __syncthreads();
     float* u = a.u + (size_t)ks * a.T * a.rank;
 #pragma unroll
     for (int i0 = 0; i0 < MT * RT; i0 += 4) {
         const int i = i0 + wave;
         if (i >= MT * RT) break;
-        const f32x4_t sum = (part[0][i][lane] + part[1][i][lane]) + (part[2][i][lane] + part[3][i][lane]);
+        const f32x4_t* p = part + i * 64 + lane;
+        const f32x4_t sum = (p[0] + p[MT * RT * 64]) + (p[2 * MT * RT * 64] + p[3 * MT * RT * 64]);
         const int tok = t.t0 + 16 * (i / RT) + row, r0 = 16 * (i % RT) + 4 * quad;
         if (tok < t.n && r0 < a.rank) *(f32x4_t*)(u + (size_t)(t.s0 + tok) * a.rank + r0) = sum;       // rank % 8 == 0
     }
@@ -134,38 +145,47 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
         }
         return;
     }
-    // U^T fragments: lane -> token col, ranks 32 k + 8 quad .. + 7
-    bf16x8_t hi[MT][KS], lo[MT][KS];
+    // U of the tile as bf16 pairs in LDS: the workgroup's threads sum the slabs of four ranks each (loads of eight slabs in
+    // flight), ranks beyond the adapter's are zero
+    constexpr int UC = 32 * KS + 8;             // padded row: the fragment reads of 16 tokens fall on different banks
+    __shared__ __attribute__((aligned(16))) __bf16 us[2][16 * MT][UC];
     const float s = a.scale ? a.scale[t.adapter] : 1.0f;
+    const size_t slab = (size_t)a.T * a.rank;
+    for (int e = threadIdx.x; e < 16 * MT * 8 * KS; e += 256) {
+        const int m = e / (8 * KS), r0 = 4 * (e % (8 * KS));
+        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+        if (r0 < a.rank) {
+            const float* up = a.u + (size_t)(t.s0 + min(t.t0 + m, t.n - 1)) * a.rank + r0;
+            for (int p = 0; p < a.ksplit; p += 8) {
+                f32x4_t w[8];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const float* up = a.u + (size_t)(t.s0 + min(t.t0 + 16 * m + col, t.n - 1)) * a.rank;
+                for (int i = 0; i < 8; ++i) w[i] = *(const f32x4_t*)(up + (size_t)min(p + i, a.ksplit - 1) * slab);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            const int r0 = 32 * k + 8 * quad;
-            f32x4_t v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
-            if (r0 < a.rank)
-                for (int p = 0; p < a.ksplit; ++p) {
-                    const f32x4_t* q = (const f32x4_t*)(up + (size_t)p * a.T * a.rank + r0);
-                    v0 += q[0];
-                    v1 += q[1];
-                }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = s * (j < 4 ? v0[j & 3] : v1[j & 3]);
-                hi[m][k][j] = (__bf16)v;
-                lo[m][k][j] = (__bf16)(v - (float)hi[m][k][j]);
+                for (int i = 0; i < 8; ++i)
+                    if (p + i < a.ksplit) v += w[i];
             }
         }
-    }
-    const char* bp = a.b + (size_t)t.adapter * a.N * a.rank * 2;
-    // 64 features a step, the four waves in turn.  Row m of weight block j is feature 16 (m >> 2) + 4 j + (m & 3): the accumulators
-    // of the four blocks then are 16 CONSECUTIVE features of a lane's token, two 16-byte pieces of R and C
-    for (int f0 = n0 + 64 * wave; f0 < n1; f0 += 256) {
-        bf16x8_t w[4][KS];
+        bf16x4_t h4, l4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int f = min(f0 + 16 * (col >> 2) + 4 * j + (col & 3), a.N - 1);
+            const float x = s * v[j];
+            h4[j] = (__bf16)x;
+            l4[j] = (__bf16)(x - (float)h4[j]);
+        }
+        *(bf16x4_t*)&us[0][m][r0] = h4;
+        *(bf16x4_t*)&us[1][m][r0] = l4;
+    }
+    const char* bp = a.b + (size_t)t.adapter * a.N * a.rank * 2;
+    // Steps of 256 features, 64 a wave.  R comes in and C goes out as contiguous 512 bytes of a row; the products meet them in an fp32
+    // LDS image [token][256] (a token's 16-byte chunks ch at ch ^ (token & 15)).
+    __shared__ __attribute__((aligned(16))) char delta[16 * MT * 1024];
+    bf16x8_t w[4][KS];
+    u32x4_t rr[2 * MT];
+    const int lr = threadIdx.x >> 5, lc = threadIdx.x & 31;
+    auto load = [&](int f0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int f = min(f0 + 64 * wave + 16 * j + col, a.N - 1);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 const int r0 = 32 * k + 8 * quad;
@@ -175,34 +195,53 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
                 w[j][k] = r0 < a.rank ? *(const bf16x8_t*)(bp + ((size_t)f * a.rank + r0) * 2) : z;
             }
         }
-        const int f = f0 + 16 * quad;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const int tok = t.t0 + 16 * m + col;
-            const bool live = tok < t.n;
-            const size_t row = t.s0 + min(tok, t.n - 1);
-            f32x4_t acc[4];
+        for (int i = 0; i < 2 * MT; ++i)
+            rr[i] = *(const u32x4_t*)(a.r + (size_t)(t.s0 + min(t.t0 + 8 * i + lr, t.n - 1)) * a.ldr_b + (size_t)min(f0 + 8 * lc, a.N - 8) * 2);
+    };
+    load(n0);                                   // flies while U is put together
+    __syncthreads();
+    bf16x8_t hi[MT][KS], lo[MT][KS];            // U^T fragments: lane -> token col, ranks 32 k + 8 quad .. + 7
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float x[8];
-                unpack8(*(const u32x4_t*)(a.r + row * a.ldr_b + (size_t)min(f + 8 * q, a.N - 8) * 2), x);
-                acc[2 * q] = (f32x4_t){x[0], x[1], x[2], x[3]};
-                acc[2 * q + 1] = (f32x4_t){x[4], x[5], x[6], x[7]};
-            }
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int k = 0; k < KS; ++k) {
+            hi[m][k] = *(const bf16x8_t*)&us[0][16 * m + col][32 * k + 8 * quad];
+            lo[m][k] = *(const bf16x8_t*)&us[1][16 * m + col][32 * k + 8 * quad];
+        }
+    for (int f0 = n0; f0 < n1; f0 += 256) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j][k], lo[m][k], acc[j], 0, 0, 0);
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j][k], hi[m][k], acc[j], 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j][k], lo[m][k], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j][k], hi[m][k], acc, 0, 0, 0);
                 }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const u32x4_t v = {pack_bf16x2(acc[2 * q][0], acc[2 * q][1]), pack_bf16x2(acc[2 * q][2], acc[2 * q][3]),
-                                   pack_bf16x2(acc[2 * q + 1][0], acc[2 * q + 1][1]), pack_bf16x2(acc[2 * q + 1][2], acc[2 * q + 1][3])};
-                if (live && f + 8 * q < n1) *(u32x4_t*)(a.c + row * a.ldc_b + (size_t)(f + 8 * q) * 2) = v;
+                // features 64 wave + 16 j + 4 quad .. + 3 of token col
+                *(f32x4_t*)(delta + (16 * m + col) * 1024 + (((16 * wave + 4 * j + quad) ^ col) << 4)) = acc;
             }
+        __syncthreads();
+        u32x4_t out[2 * MT];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+            const int tok = 8 * i + lr;
+            const f32x4_t d0 = *(const f32x4_t*)(delta + tok * 1024 + (((2 * lc) ^ (tok & 15)) << 4));
+            const f32x4_t d1 = *(const f32x4_t*)(delta + tok * 1024 + (((2 * lc + 1) ^ (tok & 15)) << 4));
+            float x[8];
+            unpack8(rr[i], x);
+            out[i] = (u32x4_t){pack_bf16x2(x[0] + d0[0], x[1] + d0[1]), pack_bf16x2(x[2] + d0[2], x[3] + d0[3]),
+                               pack_bf16x2(x[4] + d1[0], x[5] + d1[1]), pack_bf16x2(x[6] + d1[2], x[7] + d1[3])};
         }
+        if (f0 + 256 < n1) load(f0 + 256);
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+            const int tok = t.t0 + 8 * i + lr;
+            if (tok < t.n && f0 + 8 * lc < n1) *(u32x4_t*)(a.c + (size_t)(t.s0 + tok) * a.ldc_b + (size_t)(f0 + 8 * lc) * 2) = out[i];
+        }
+        __syncthreads();
     }
 }
 
@@ -213,19 +252,21 @@ struct Plan {
 
 Plan make_plan(int T, int B, int N, int K, int rank, int cus) {
     Plan p;
-    const double rho = (double)T / B;                           // tokens per sequence, on average
-    p.mt = rho <= 16 ? 1 : rho <= 32 || rank > 64 ? 2 : 4;
+    // 16 tokens a tile where sequences have no more on average, else 32: 64 measured slower (prompts of up to 1024 tokens, rank 32,
+    // 2048 -> 6144: 113 us with 32, 128 with 64, 124 with 16: fewer workgroups fit a CU)
+    p.mt = (double)T / B <= 16 ? 1 : 2;
     p.nslots = (long long)T / (16 * p.mt) + B;
     const long long tiles = ((long long)T + 16 * p.mt - 1) / (16 * p.mt) > B ? ((long long)T + 16 * p.mt - 1) / (16 * p.mt) : B;
-    // two workgroups per CU, no K range shorter than the four waves' steps
-    long long ks = (2LL * cus + tiles - 1) / tiles;
+    // K ranges: one workgroup per CU (every slab is read again by every slice of the second launch: 32 blocks of 32 tokens, rank 64,
+    // 6144 -> 2048 took 22.4 us so, 27.6 with two per CU), no range under one step of the four waves
+    long long ks = (cus + tiles - 1) / tiles;
     if (ks > K / 256) ks = K / 256;
     if (ks < 1) ks = 1;
     p.kchunk = (int)(((K + ks - 1) / ks + 63) / 64 * 64);
     p.ksplit = (K + p.kchunk - 1) / p.kchunk;
-    // features of a workgroup: 256 (one step of each wave), more when that still makes eight workgroups per CU
-    p.nslice = 256;
-    while (p.nslice < 1024 && p.nslice < N && tiles * ((N + 2 * p.nslice - 1) / (2 * p.nslice)) >= 8LL * cus) p.nslice *= 2;
+    // features of a workgroup: two steps where that leaves a workgroup per CU (U is put together once for both: 135 us against 143 on the
+    // prompts above, and four steps 138), else one
+    p.nslice = tiles * ((N + 511) / 512) >= cus ? 512 : 256;
     return p;
 }
 
@@ -264,22 +305,26 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
     a.u = (float*)workspace;
     hipStream_t st = (hipStream_t)stream;
     const dim3 gd((unsigned)downs), gu((unsigned)ups), block(256);
-    const int rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
-#define CODA_LORA_RANKS(MT)                                                                             \
-    do {                                                                                                \
-        if (rt == 1) hipLaunchKernelGGL((lora_down_kernel<MT, 1>), gd, block, 0, st, a);                \
-        else if (rt == 2) hipLaunchKernelGGL((lora_down_kernel<MT, 2>), gd, block, 0, st, a);           \
-        else if (rt == 4) hipLaunchKernelGGL((lora_down_kernel<MT, 4>), gd, block, 0, st, a);           \
-        else hipLaunchKernelGGL((lora_down_kernel<(MT > 2 ? 2 : MT), 8>), gd, block, 0, st, a);         \
-        CODA_CHECK_LAUNCH("lora down");                                                                 \
-        if (rt <= 2) hipLaunchKernelGGL((lora_up_kernel<MT, 1>), gu, block, 0, st, a);                  \
-        else if (rt == 4) hipLaunchKernelGGL((lora_up_kernel<MT, 2>), gu, block, 0, st, a);             \
-        else hipLaunchKernelGGL((lora_up_kernel<(MT > 2 ? 2 : MT), 4>), gu, block, 0, st, a);           \
-        CODA_CHECK_LAUNCH("lora up");                                                                   \
-    } while (0)
-    if (p.mt == 1) CODA_LORA_RANKS(1);
-    else if (p.mt == 2) CODA_LORA_RANKS(2);
-    else CODA_LORA_RANKS(4);                    // rank <= 64: make_plan gives larger ranks at most 32 tokens a tile
-#undef CODA_LORA_RANKS
-    return CODA_OK;
+    auto down = [&](auto kernel, int lds) -> int {
+        if (coda_ensure_dyn_lds((const void*)kernel, lds) != CODA_OK) return CODA_ERR_LAUNCH;
+        hipLaunchKernelGGL(kernel, gd, block, lds, st, a);
+        CODA_CHECK_LAUNCH("lora down");
+        return CODA_OK;
+    };
+    // ranks in blocks of 16 (down) and 32 (up)
+    auto go = [&](auto mt) -> int {
+        constexpr int MT = decltype(mt)::value;
+        int rc;
+        if (rank <= 16) rc = down(lora_down_kernel<MT, 1>, Down<MT, 1>::LDS);
+        else if (rank <= 32) rc = down(lora_down_kernel<MT, 2>, Down<MT, 2>::LDS);
+        else if (rank <= 64) rc = down(lora_down_kernel<MT, 4>, Down<MT, 4>::LDS);
+        else rc = down(lora_down_kernel<MT, 8>, Down<MT, 8>::LDS);
+        if (rc != CODA_OK) return rc;
+        if (rank <= 32) hipLaunchKernelGGL((lora_up_kernel<MT, 1>), gu, block, 0, st, a);
+        else if (rank <= 64) hipLaunchKernelGGL((lora_up_kernel<MT, 2>), gu, block, 0, st, a);
+        else hipLaunchKernelGGL((lora_up_kernel<MT, 4>), gu, block, 0, st, a);
+        CODA_CHECK_LAUNCH("lora up");
+        return CODA_OK;
+    };
+    return p.mt == 1 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
 }

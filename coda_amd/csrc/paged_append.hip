@@ -79,12 +79,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     const long long wave = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const long long tl = wave / a.parts;
     if (tl >= a.T) return;
-    const int t = (int)tl, part = (int)(wave - tl * a.parts);
-    const int b = wave_search(a.B, t, [&](int i) { return (long long)a.seq_start[i]; });
-    if (b < 0) return;
-    const int s0 = a.seq_start[b];
-    if (t >= a.seq_start[b + 1]) return;                        // a row of no sequence: left alone
-    const long long p64 = (long long)a.pos0[b] + ((long long)t - s0);
+    const int t = __builtin_amdgcn_readfirstlane((int)tl), part = __builtin_amdgcn_readfirstlane((int)(wave - tl * a.parts));
+    const Seq q = seq_of_token({a.seq_start, a.pos0, nullptr, a.B, a.T}, t);
+    if (q.b < 0) return;                                        // a row of no sequence: left alone
+    const int b = q.b;
+    const long long p64 = (long long)q.x + (t - q.s0);
     if (p64 < 0 || p64 >= a.max_pos) return;                    // no rotary row: nothing is written for this token
     const int pos = (int)p64;
     const int lp = fast_div(a.pg.page, pos), slot = pos - lp * (int)a.pg.page.d;

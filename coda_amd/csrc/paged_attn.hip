@@ -2,9 +2,9 @@
 //
 //     out_i = sum_j softmax_j(scale q_i . K_j) V_j over the keys j < lim(i) of the token's sequence
 //
-// One pass over the keys with a running maximum and sum (in log2 units); the keys are cut into `nsplit` ranges where there
-// are too few rows to fill the chip, and a second kernel joins the ranges' (maximum, sum, unnormalised output) triples in
-// fp32, in a fixed order.
+// One pass over the keys with a running maximum and sum (in log2 units).  Where there are too few rows to fill the chip, or rows of
+// very different lengths, the keys are cut into ranges and a second kernel joins the ranges' (maximum, sum, unnormalised output)
+// triples in fp32, in a fixed order.  How long a range is comes from the lengths on the device (see cut_of): the host knows only bounds.
 //
 // Rows.  The g = n_q / n_kv query heads of a key/value head read the same keys, so a sequence of n tokens is n g ROWS per
 // key/value head (row r = token r / g, head r % g) and tiles are cut from those: one token of a g = 2 model is two rows of one
@@ -27,7 +27,6 @@ using namespace paged;
 namespace {
 
 constexpr float RESCALE_THR = 6.0f;            // log2 units: weights stay below 2^6 between rescales
-constexpr int MAX_SPLITS = 256;
 
 struct AttnArgs {
     const char* q; long long ldq_b;
@@ -40,44 +39,73 @@ struct AttnArgs {
     FastDiv gdiv;
     int mask_block;
     float scale_log2e, v_scale;
-    int nslots, nsplit, split_len;
-    float* po; float* pml;                     // partial outputs [nsplit][T n_q][128] and (maximum, sum) [nsplit][T n_q][2]
+    int max_ranges;                            // 1: keys are not cut
+    int min_keys; float per_range;             // a range: at least min_keys keys, and sum(tiles * keys) * per_range
+    float* po; float* pml;                     // partial outputs [max_ranges][T n_q][128] and (maximum, sum) [max_ranges][T n_q][2]
+    int* range_keys;                           // the range length that the first kernel took, for the second
 };
 
 __device__ __forceinline__ int swz(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
 
 typedef __attribute__((ext_vector_type(8))) short s16x8_t;
 
-// A tile of `R` rows of one sequence: tile slots are numbered so that sequence b owns floor(start_b g / R) + b onwards, which
-// needs no prefix sum over the sequences and leaves each at least ceil(n g / R) slots (a slot beyond its rows is idle).
+// A tile of R rows of one sequence and a range of its keys; what its rows see: all of the sequence's kv keys, or those before the end
+// of the row's mask block.
 struct TileRows {
     int b, s0, n;        // sequence, its first token row, its tokens
     int r0, rows;        // first row of the tile, rows of the sequence
+    int range, keys;     // range of keys and its length
 };
 
-template <int R>
-__device__ __forceinline__ bool find_tile(const AttnArgs& a, int slot, TileRows& t) {
-    auto first = [&](int i) { return (long long)clamp_start(a.seq_start, i, a.T) * a.g / R + i; };
-    t.b = wave_search(a.B, slot, first);
-    if (t.b < 0) return false;
-    t.s0 = clamp_start(a.seq_start, t.b, a.T);
-    t.n = clamp_start(a.seq_start, t.b + 1, a.T) - t.s0;
-    t.rows = t.n * a.g;
-    const long long r0 = (slot - first(t.b)) * R;
-    t.r0 = (int)r0;
-    return r0 < t.rows;
-}
-
-// Keys that token i of the sequence sees: all of its kv_len, or those before the end of the token's mask block.
 struct Limits {
     int kv; long long pos0;
 };
 
-__device__ __forceinline__ Limits load_limits(const AttnArgs& a, int b) {
-    Limits l;
-    l.kv = min(max(a.kv_len[b], 0), a.max_kv);
-    l.pos0 = a.mask_block ? a.pos0[b] : 0;
-    return l;
+__device__ __forceinline__ int kv_of(const AttnArgs& a, int x) { return min(max(x, 0), a.max_kv); }
+
+__device__ __forceinline__ Limits limits_of(const AttnArgs& a, const Seq& q) { return {kv_of(a, q.x), q.y}; }
+
+// Length of the ranges of a sequence with kv keys: ceil(kv / range_keys) equal ones, in whole 128 keys
+__device__ __forceinline__ int keys_of(int kv, int range_keys) {
+    const int n = max(1, (kv + range_keys - 1) / range_keys);
+    return ((kv + n - 1) / n + 127) & ~127;
+}
+
+// Work unit -> tile and range.  The longest a range may be follows from the whole work, sum over the sequences of tiles * keys, so that
+// the units come out about equal and about as many as the chip takes at once (or in a few rounds): every wave adds the lengths up for
+// itself, in the same order.
+template <int R>
+__device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, TileRows& t, Limits& lm) {
+    const SeqArrays arr = {a.seq_start, a.kv_len, a.pos0, a.B, a.T};
+    SeqBlock blk;
+    blk.load(arr, 0);
+    int range_keys = 0x40000000;
+    if (a.max_ranges > 1) {
+        float work = 0.f;
+        for (int c = 0; c < a.B; c += 256) {
+            SeqBlock more;
+            if (c) more.load(arr, c);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const SeqLane& l = c ? more.l[u] : blk.l[u];
+                work += (float)tiles_of<R>(l, a.g) * (float)kv_of(a, l.x);
+            }
+        }
+        work = wave_sum(work);
+        range_keys = max(a.min_keys, ((int)fminf(work * a.per_range, 1e9f) + 128) & ~127);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.range_keys = range_keys;
+    }
+    int k;
+    const Seq q = seq_of_item(arr, blk, unit, k, [&](const SeqLane& l) {
+        const int kv = kv_of(a, l.x);
+        return tiles_of<R>(l, a.g) * (a.max_ranges > 1 ? max(1, (kv + range_keys - 1) / range_keys) : 1);
+    });
+    if (q.b < 0) return false;
+    lm = limits_of(a, q);
+    const int rows = q.n * a.g, tiles = rows / R + (rows % R != 0), ranges = max(1, (lm.kv + range_keys - 1) / range_keys);
+    // later tiles see more keys under a mask: they go first
+    t = {q.b, q.s0, q.n, (tiles - 1 - k / ranges) * R, rows, k % ranges, keys_of(lm.kv, range_keys)};
+    return true;
 }
 
 __device__ __forceinline__ int limit_of(const AttnArgs& a, const Limits& l, int token) {
@@ -123,32 +151,33 @@ struct TileSource {
     int first;
     size_t base[G16 ? NP : 1];                 // G16: of each piece's group (uniform); else: of key lane & (KEYS - 1)
     unsigned long long ok;                     // keys that exist
-    int entry[G16 ? GROUPS : 1], mine[G16 ? NP : 1];      // page numbers of the tile looked up last: of every group, of this wave's pieces
+    int entry;                                 // page number of the tile looked up last, lane l: of group l (G16) or key l
 
-    __device__ __forceinline__ int group_key(int i) const { return ((i * STRIDE + first) * PROWS) & ~15; }
+    // a vector load also where all lanes want few numbers: a scalar one would be waited for with the next LDS read, a tile early
     __device__ __forceinline__ void look_up(const AttnArgs& a, const int* table, int key0, int end) {
-        if (G16) {
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) entry[g] = page_entry(a, table, key0 + 16 * g, end);
-#pragma unroll
-            for (int i = 0; i < NP; ++i) mine[i] = page_entry(a, table, key0 + group_key(i), end);
-        } else {
-            entry[0] = page_entry(a, table, key0 + (int)(threadIdx.x & (KEYS - 1)), end);
-        }
+        const int lane = threadIdx.x & 63;
+        entry = page_entry(a, table, key0 + (G16 ? 16 * (lane & (GROUPS - 1)) : lane & (KEYS - 1)), end);
     }
     // page numbers -> offsets, for the tile that look_up was last called for
     __device__ __forceinline__ void resolve(const AttnArgs& a, int key0, int end) {
+        const int lane = threadIdx.x & 63;
         if (G16) {
+            const int key = key0 + 16 * (lane & (GROUPS - 1));
+            const KeyAt at = key_at(a, entry, key);
             ok = 0;
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                const int live = (unsigned)entry[g] < (unsigned)a.pg.num_pages ? min(max(end - key0 - 16 * g, 0), 16) : 0;
+                const int live = __builtin_amdgcn_readlane((int)at.ok, g) ? min(max(end - key0 - 16 * g, 0), 16) : 0;
                 ok |= (unsigned long long)((1u << live) - 1u) << (16 * g);
             }
 #pragma unroll
-            for (int i = 0; i < NP; ++i) base[i] = key_at(a, mine[i], key0 + group_key(i)).off;
+            for (int i = 0; i < NP; ++i) {
+                const int g = (i * STRIDE + first) * PROWS / 16;
+                const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)at.off, g), hi = __builtin_amdgcn_readlane((int)(unsigned)(at.off >> 32), g);
+                base[i] = ((size_t)hi << 32) | lo;
+            }
         } else {
-            const KeyAt at = key_at(a, entry[0], key0 + (int)(threadIdx.x & (KEYS - 1)));
+            const KeyAt at = key_at(a, entry, key0 + (lane & (KEYS - 1)));
             ok = __ballot(at.ok);
             if (KEYS < 64) ok &= (1ull << (KEYS & 63)) - 1;
             base[0] = at.off;
@@ -325,16 +354,16 @@ __global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(At
     __shared__ float ml[4][2][R];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
-    const int slot = blockIdx.x % a.nslots, kvh = (blockIdx.x / a.nslots) % a.n_kv, split = blockIdx.x / (a.nslots * a.n_kv);
+    const int kvh = blockIdx.x % a.n_kv;
     TileRows tr;
-    if (!find_tile<R>(a, slot, tr)) return;
-    const Limits lm = load_limits(a, tr.b);
+    Limits lm;
+    if (!find_unit<R>(a, blockIdx.x / a.n_kv, tr, lm)) return;
     const int last = min(tr.r0 + R, tr.rows) - 1;               // last live row of the tile
     const int end = limit_of(a, lm, fast_div(a.gdiv, last));    // keys that any row of the tile sees
     const int all = limit_of(a, lm, fast_div(a.gdiv, tr.r0));   // keys that every row of it sees
-    const int nsp = max(1, (end + a.split_len - 1) / a.split_len);
-    if (split >= nsp) return;
-    const int k_lo = split * a.split_len, k_hi = min(end, k_lo + a.split_len);
+    const int nsp = a.max_ranges > 1 ? max(1, (end + tr.keys - 1) / tr.keys) : 1;
+    if (tr.range >= nsp) return;
+    const int k_lo = tr.range * tr.keys, k_hi = min(end, k_lo + tr.keys);
     const size_t head_off = (size_t)kvh * a.pg.head_stride_b;
     const int* table = a.pg.table + (size_t)tr.b * a.pg.ld_table;
     const char* kbase = a.k + head_off;
@@ -554,7 +583,7 @@ __global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(At
                 *(u32x4_t*)(op + q8 * 16) = pack8(y);
             }
         } else {
-            const size_t row = (size_t)split * a.T * a.n_q + (size_t)at.token * a.n_q + at.head;
+            const size_t row = (size_t)tr.range * a.T * a.n_q + (size_t)at.token * a.n_q + at.head;
             float* op = a.po + row * HEAD_DIM + ch0 * 4;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) *(f32x4_t*)(op + 4 * q4) = (f32x4_t){acc[4 * q4], acc[4 * q4 + 1], acc[4 * q4 + 2], acc[4 * q4 + 3]};
@@ -576,18 +605,18 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
     __shared__ int dropped_s[4];                                // tile t & 3: non-finite values were dropped from its V image
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
-    // tiles of a sequence read the same keys: consecutive slots of one head run on one XCD and share its L2
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int slot = id % a.nslots, kvh = (id / a.nslots) % a.n_kv, split = id / (a.nslots * a.n_kv);
+    // tiles of a sequence read the same keys: with the key/value head as the fastest index, and workgroups going round the eight XCDs, a
+    // head stays on few XCDs (one, for 8 heads) and its keys are found in that L2
+    const int kvh = blockIdx.x % a.n_kv;
     TileRows tr;
-    if (!find_tile<R>(a, slot, tr)) return;
-    const Limits lm = load_limits(a, tr.b);
+    Limits lm;
+    if (!find_unit<R>(a, blockIdx.x / a.n_kv, tr, lm)) return;
     const int last = min(tr.r0 + R, tr.rows) - 1;
     const int end = limit_of(a, lm, fast_div(a.gdiv, last));
     const int all = limit_of(a, lm, fast_div(a.gdiv, tr.r0));
-    const int nsp = max(1, (end + a.split_len - 1) / a.split_len);
-    if (split >= nsp) return;
-    const int k_lo = split * a.split_len, k_hi = min(end, k_lo + a.split_len);
+    const int nsp = a.max_ranges > 1 ? max(1, (end + tr.keys - 1) / tr.keys) : 1;
+    if (tr.range >= nsp) return;
+    const int k_lo = tr.range * tr.keys, k_hi = min(end, k_lo + tr.keys);
     const size_t head_off = (size_t)kvh * a.pg.head_stride_b;
     const int* table = a.pg.table + (size_t)tr.b * a.pg.ld_table;
     const char* kbase = a.k + head_off;
@@ -767,7 +796,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
                 if (live) *(u32x4_t*)(op + (32 * db + 8 * (2 * j + h)) * 2) = (u32x4_t){s0[0], s1[0], s0[1], s1[1]};
             }
     } else if (live) {
-        const size_t row = (size_t)split * a.T * a.n_q + (size_t)at.token * a.n_q + at.head;
+        const size_t row = (size_t)tr.range * a.T * a.n_q + (size_t)at.token * a.n_q + at.head;
         float* op = a.po + row * HEAD_DIM;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
@@ -779,36 +808,85 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Joins the ranges of one (token, head) row: 32 lanes hold its 128 features, the 8 half-waves of the workgroup take ranges in
-// turn and meet in LDS.  R: rows per tile of the kernel that wrote the ranges (a tile's rows have the same number of ranges).
+// Joins the key ranges of (token, head) rows.  R: rows per tile of the kernel that wrote the ranges (the rows of a tile have the same
+// number of ranges).  Up to FEW_RANGES ranges: a wave per row, every range's loads in flight at once; more: a workgroup per row, the
+// ranges shared out over its eight half-waves, which meet in LDS.
+constexpr int FEW_RANGES = 8;
+
+// weight of a part with maximum m in a sum with maximum mm; a part without a maximum holds zeros (or NaN): nothing to scale
+__device__ __forceinline__ float part_weight(float m, float mm) { return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mm); }
+
+template <int R>
+__device__ __forceinline__ int ranges_of(const AttnArgs& a, int token, int head) {
+    const Seq q = seq_of_token({a.seq_start, a.kv_len, a.pos0, a.B, a.T}, token);
+    if (q.b < 0) return 0;                                      // a row of no sequence
+    const int r = (token - q.s0) * a.g + head % a.g;
+    const int last = (int)min(((long long)r / R + 1) * R, (long long)q.n * a.g) - 1;
+    const Limits lm = limits_of(a, q);
+    const int end = limit_of(a, lm, fast_div(a.gdiv, last)), keys = keys_of(lm.kv, *a.range_keys);
+    return (end + keys - 1) / keys;
+}
+
+template <int R>
+__global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int row = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
+    const int rows = a.T * a.n_q;
+    if (row >= rows) return;
+    const int token = row / a.n_q, head = row % a.n_q;
+    const int nsp = ranges_of<R>(a, token, head);
+    if (nsp <= 1) return;                                       // written by the first kernel
+    f32x2_t e[FEW_RANGES], x[FEW_RANGES];
+#pragma unroll
+    for (int i = 0; i < FEW_RANGES; ++i) {
+        const size_t at = (size_t)min(i, nsp - 1) * rows + row;
+        e[i] = *(const f32x2_t*)(a.pml + at * 2);
+        x[i] = *(const f32x2_t*)(a.po + at * HEAD_DIM + 2 * lane);
+    }
+    float mm = -INFINITY, tot = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < FEW_RANGES; ++i) mm = fmaxf(mm, e[i][0]);
+#pragma unroll
+    for (int i = 0; i < FEW_RANGES; ++i) {
+        if (i >= nsp) break;
+        const float f = part_weight(e[i][0], mm);
+        tot += e[i][1] * f;
+        y0 += x[i][0] * f;
+        y1 += x[i][1] * f;
+    }
+    const float inv = tot == 0.f ? 0.f : a.v_scale / tot;
+    *(unsigned int*)(a.out + (size_t)token * a.ldo_b + (size_t)head * 256 + lane * 4) = pack_bf16x2(y0 * inv, y1 * inv);
+}
+
 template <int R>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
     __shared__ float sm[8], sl[8];
     __shared__ f32x4_t so[8][32];
     const int token = blockIdx.x / a.n_q, head = blockIdx.x % a.n_q;
-    const int b = wave_search(a.B, token, [&](int i) { return (long long)clamp_start(a.seq_start, i, a.T); });
-    if (b < 0) return;
-    const int s0 = clamp_start(a.seq_start, b, a.T), n = clamp_start(a.seq_start, b + 1, a.T) - s0;
-    if (token - s0 >= n) return;                                // a row of no sequence
-    const int r = (token - s0) * a.g + head % a.g;
-    const int last = (int)min(((long long)r / R + 1) * R, (long long)n * a.g) - 1;
-    const Limits lm = load_limits(a, b);
-    const int end = limit_of(a, lm, fast_div(a.gdiv, last));
-    const int nsp = (end + a.split_len - 1) / a.split_len;
-    if (nsp <= 1) return;                                       // written by the first kernel
+    const int nsp = ranges_of<R>(a, token, head);
+    if (nsp <= 1) return;
     const int grp = threadIdx.x >> 5, l = threadIdx.x & 31;
     const size_t rows = (size_t)a.T * a.n_q, row = (size_t)blockIdx.x;
     float m = -INFINITY, sum = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = grp; s < nsp; s += 8) {
-        const f32x2_t e = *(const f32x2_t*)(a.pml + (s * rows + row) * 2);
-        const f32x4_t x = *(const f32x4_t*)(a.po + (s * rows + row) * HEAD_DIM + 4 * l);
-        const float mn = fmaxf(m, e[0]);                        // -inf: no key of the range was seen, sums of 0
-        const float fo = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        const float fn = e[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(e[0] - mn);
-        sum = sum * fo + e[1] * fn;
-        acc = acc * fo + x * fn;
-        m = mn;
+    for (int s0 = grp; s0 < nsp; s0 += 32) {                    // four ranges in flight
+        f32x2_t e[4];
+        f32x4_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const size_t at = (size_t)min(s0 + 8 * i, nsp - 1) * rows + row;
+            e[i] = *(const f32x2_t*)(a.pml + at * 2);
+            x[i] = *(const f32x4_t*)(a.po + at * HEAD_DIM + 4 * l);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + 8 * i >= nsp) break;
+            const float mn = fmaxf(m, e[i][0]);
+            const float fo = part_weight(m, mn), fn = part_weight(e[i][0], mn);
+            sum = sum * fo + e[i][1] * fn;
+            acc = acc * fo + x[i] * fn;
+            m = mn;
+        }
     }
     if (l == 0) { sm[grp] = m; sl[grp] = sum; }
     so[grp][l] = acc;
@@ -821,7 +899,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
     f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float f = sm[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[i] - mm);
+        const float f = part_weight(sm[i], mm);
         tot += sl[i] * f;
         y = y + so[i][l] * f;
     }
@@ -830,32 +908,42 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
         (u32x2_t){pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
 }
 
-// How a call is cut: rows per tile, tile slots, key ranges.  A function of the call's sizes alone.
+// How a call is cut: rows per tile, workgroups, the bounds of the key ranges.  A function of the call's sizes alone.
 struct Plan {
-    int R; long long nslots; int nsplit, split_len;
+    int R; long long wgs; int max_ranges, min_keys; float per_range;
 };
+
+constexpr int WS_HEAD = 256;                    // bytes in front of the partial outputs: the range length
 
 Plan make_plan(int T, int B, int max_kv, int n_q, int n_kv, int cus) {
     const int g = n_q / n_kv;
     const double rho = (double)T * g / B;                       // rows per sequence and key/value head, on average
     Plan p;
     p.R = rho <= 32 ? 32 : rho <= 64 ? 64 : rho <= 128 ? 128 : 256;
-    p.nslots = (long long)T * g / p.R + B;
-    // ranges: enough workgroups for two per CU (one where a workgroup has the CU to itself), none shorter than 256 keys
-    const long long tiles = (((long long)T * g + p.R - 1) / p.R > B ? ((long long)T * g + p.R - 1) / p.R : B) * n_kv;
-    const long long want = (p.R == 32 || p.R == 128 ? 2 : 1) * (long long)cus;
-    long long ns = (want + tiles - 1) / tiles;
-    const long long most = (max_kv + 255) / 256;
-    if (ns > most) ns = most;
-    if (ns > MAX_SPLITS) ns = MAX_SPLITS;
-    if (ns < 1) ns = 1;
-    p.split_len = max_kv > 0 ? (int)((max_kv + ns - 1) / ns) : 1;
-    p.split_len = (p.split_len + 127) / 128 * 128;
-    p.nsplit = max_kv > 0 ? (max_kv + p.split_len - 1) / p.split_len : 1;
+    const long long bound = (long long)T * g / p.R + B;         // tiles per key/value head, at most
+    const long long some = ((long long)T * g + p.R - 1) / p.R > B ? ((long long)T * g + p.R - 1) / p.R : B;   // and where no sequence is empty, at least
+    const long long slots = (p.R == 32 || p.R == 128 ? 2 : 1) * (long long)cus;          // workgroups resident at once
+    // no range under eight steps of a workgroup (the second kernel and a short range's start cost as much), and no more partial outputs
+    // than 64 MiB
+    const int least = p.R <= 64 ? 1024 : 512;
+    const long long row_bytes = (long long)T * n_q * (HEAD_DIM + 2) * 4;
+    long long most = max_kv / least;
+    if (most > (64LL << 20) / row_bytes) most = (64LL << 20) / row_bytes;
+    if (most > 256) most = 256;
+    // few tiles: one round of equal units.  Many: about four rounds, so that sequences of unequal length even out
+    const long long units = some * n_kv * 2 <= slots ? slots - some * n_kv : 4 * slots;
+    p.max_ranges = most < 2 || some * n_kv >= 2 * units ? 1 : (int)most;
+    p.min_keys = p.max_ranges > 1 ? ((max_kv + p.max_ranges - 1) / p.max_ranges + 127) / 128 * 128 : 0;
+    if (p.max_ranges > 1 && p.min_keys < least) p.min_keys = least;
+    p.per_range = (float)((double)n_kv / units);
+    // every tile's first range, and the further ones: at most work / range length <= units / n_kv of them (1/64 for the sum's rounding)
+    p.wgs = bound * n_kv + (p.max_ranges > 1 ? units + units / 64 + n_kv : 0);
     return p;
 }
 
-long long plan_bytes(const Plan& p, int T, int n_q) { return p.nsplit > 1 ? (long long)p.nsplit * T * n_q * (HEAD_DIM + 2) * 4 : 0; }
+long long plan_bytes(const Plan& p, int T, int n_q) {
+    return p.max_ranges > 1 ? WS_HEAD + (long long)p.max_ranges * T * n_q * (HEAD_DIM + 2) * 4 : 0;
+}
 
 }  // namespace
 
@@ -886,8 +974,7 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     const long long need = plan_bytes(p, T, n_q);
     if (need > 0 && (!workspace || workspace_bytes < need)) return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_paged_attn_workspace_bytes");
     if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
-    const long long wgs = p.nslots * n_kv * p.nsplit;
-    if (wgs > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
+    if (p.wgs > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
     const bool f8 = cache_type == CODA_CACHE_E4M3;
     a.q = (const char*)q; a.ldq_b = ld_q * 2;
     a.out = (char*)out; a.ldo_b = ld_out * 2;
@@ -898,13 +985,14 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     a.mask_block = mask_block;
     a.scale_log2e = scale * (f8 ? k_scale : 1.0f) * 1.4426950408889634f;
     a.v_scale = f8 ? v_scale : 1.0f;
-    a.nslots = (int)p.nslots; a.nsplit = p.nsplit; a.split_len = p.split_len;
-    a.po = (float*)workspace;
-    a.pml = p.nsplit > 1 ? (float*)workspace + (long long)p.nsplit * T * n_q * HEAD_DIM : nullptr;
+    a.max_ranges = p.max_ranges; a.min_keys = p.min_keys; a.per_range = p.per_range;
+    a.range_keys = p.max_ranges > 1 ? (int*)workspace : nullptr;
+    a.po = p.max_ranges > 1 ? (float*)((char*)workspace + WS_HEAD) : nullptr;
+    a.pml = p.max_ranges > 1 ? a.po + (long long)p.max_ranges * T * n_q * HEAD_DIM : nullptr;
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto kernel, int threads, int lds) -> int {
         if (coda_ensure_dyn_lds((const void*)kernel, lds) != CODA_OK) return CODA_ERR_LAUNCH;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(threads), lds, st, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)p.wgs), dim3(threads), lds, st, a);
         CODA_CHECK_LAUNCH("paged_attn");
         return CODA_OK;
     };
@@ -920,12 +1008,17 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     const std::true_type yes{};
     const std::false_type no{};
     const int r2 = f8 ? (g16 ? pick(yes, yes) : pick(yes, no)) : (g16 ? pick(no, yes) : pick(no, no));
-    if (r2 != CODA_OK || p.nsplit == 1) return r2;
-    const dim3 jg((unsigned)((long long)T * n_q));
-    if (p.R == 32) hipLaunchKernelGGL(paged_attn_join_kernel<32>, jg, dim3(256), 0, st, a);
-    else if (p.R == 64) hipLaunchKernelGGL(paged_attn_join_kernel<64>, jg, dim3(256), 0, st, a);
-    else if (p.R == 128) hipLaunchKernelGGL(paged_attn_join_kernel<128>, jg, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(paged_attn_join_kernel<256>, jg, dim3(256), 0, st, a);
+    if (r2 != CODA_OK || p.max_ranges == 1) return r2;
+    const long long rows = (long long)T * n_q;
+    auto join = [&](auto tile_rows) {
+        constexpr int R = decltype(tile_rows)::value;
+        if (p.max_ranges <= FEW_RANGES) hipLaunchKernelGGL(paged_attn_join_few_kernel<R>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(paged_attn_join_kernel<R>, dim3((unsigned)rows), dim3(256), 0, st, a);
+    };
+    if (p.R == 32) join(std::integral_constant<int, 32>{});
+    else if (p.R == 64) join(std::integral_constant<int, 64>{});
+    else if (p.R == 128) join(std::integral_constant<int, 128>{});
+    else join(std::integral_constant<int, 256>{});
     CODA_CHECK_LAUNCH("paged_attn join");
     return CODA_OK;
 }
