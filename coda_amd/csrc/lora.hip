@@ -18,6 +18,12 @@ using namespace paged;
 
 namespace {
 
+struct Tile {
+    int row0, n;                                // first token row, tokens (0: there is no such tile)
+    int adapter;                                // -1: none
+    int unused;
+};
+
 struct LoraArgs {
     const char* x; long long ldx_b;
     const char* a; const char* b;
@@ -29,22 +35,18 @@ struct LoraArgs {
     int N, K;
     int nslots, ksplit, kchunk, nslice;
     float* u;                                   // [ksplit][T][rank]
-};
-
-struct Tile {
-    int b, s0, n, t0, adapter;                  // sequence, its first row, its tokens; the tile's first token; -1: no adapter
+    Tile* tiles;                                // [nslots]: what the first launch found, for the second
 };
 
 template <int TM>
-__device__ __forceinline__ bool find_tile(const LoraArgs& a, int slot, Tile& t) {
+__device__ __forceinline__ Tile find_tile(const LoraArgs& a, int slot) {
     const SeqArrays arr = {a.seq_start, a.adapter, nullptr, a.B, a.T};
     SeqBlock blk;
     blk.load(arr, 0);
     int k;
     const Seq q = seq_of_item(arr, blk, slot, k, [](const SeqLane& l) { return tiles_of<TM>(l, 1); });
-    if (q.b < 0) return false;
-    t = {q.b, q.s0, q.n, k * TM, (unsigned)q.x < (unsigned)a.n_adapters ? q.x : -1};
-    return true;
+    if (q.b < 0) return {0, 0, -1, 0};
+    return {q.s0 + k * TM, min(q.n - k * TM, TM), (unsigned)q.x < (unsigned)a.n_adapters ? q.x : -1, 0};
 }
 
 // U of 16 MT tokens, 16 RT ranks (those beyond the adapter's are computed from its last row and dropped).
@@ -63,14 +65,15 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     constexpr int NL = Down<MT, RT>::NL;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = blockIdx.x / a.ksplit, ks = blockIdx.x % a.ksplit;
-    Tile t;
-    if (!find_tile<16 * MT>(a, slot, t) || t.adapter < 0) return;
+    const Tile t = find_tile<16 * MT>(a, slot);
+    if (ks == 0 && threadIdx.x == 0) a.tiles[slot] = t;
+    if (t.n == 0 || t.adapter < 0) return;
     const int lr = threadIdx.x >> 5, lc = threadIdx.x & 31;     // this thread's row (of 8) and chunk in a pass
     const char* src[NL];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
         const int r = 8 * i + lr;
-        src[i] = (i < 2 * MT ? a.x + (size_t)(t.s0 + min(t.t0 + r, t.n - 1)) * a.ldx_b
+        src[i] = (i < 2 * MT ? a.x + (size_t)(t.row0 + min(r, t.n - 1)) * a.ldx_b
                              : a.a + ((size_t)t.adapter * a.rank + min(r - 16 * MT, a.rank - 1)) * a.K * 2);
     }
     const int k0 = ks * a.kchunk, k1 = min(a.K, k0 + a.kchunk);
@@ -122,8 +125,8 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
         if (i >= MT * RT) break;
         const f32x4_t* p = part + i * 64 + lane;
         const f32x4_t sum = (p[0] + p[MT * RT * 64]) + (p[2 * MT * RT * 64] + p[3 * MT * RT * 64]);
-        const int tok = t.t0 + 16 * (i / RT) + row, r0 = 16 * (i % RT) + 4 * quad;
-        if (tok < t.n && r0 < a.rank) *(f32x4_t*)(u + (size_t)(t.s0 + tok) * a.rank + r0) = sum;       // rank % 8 == 0
+        const int tok = 16 * (i / RT) + row, r0 = 16 * (i % RT) + 4 * quad;
+        if (tok < t.n && r0 < a.rank) *(f32x4_t*)(u + (size_t)(t.row0 + tok) * a.rank + r0) = sum;       // rank % 8 == 0
     }
 }
 
@@ -133,47 +136,17 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nsl = (a.N + a.nslice - 1) / a.nslice;
     const int slot = blockIdx.x / nsl, n0 = (blockIdx.x % nsl) * a.nslice, n1 = min(a.N, n0 + a.nslice);
-    Tile t;
-    if (!find_tile<16 * MT>(a, slot, t)) return;
+    const Tile t = a.tiles[slot];
+    if (t.n == 0) return;
     const int col = lane & 15, quad = lane >> 4;
     if (t.adapter < 0) {
         if (a.r == a.c && a.ldr_b == a.ldc_b) return;
-        for (int m = 0; m < 16 * MT && t.t0 + m < t.n; ++m) {
-            const size_t row = t.s0 + t.t0 + m;
+        for (int m = 0; m < t.n; ++m) {
+            const size_t row = t.row0 + m;
             for (int f = n0 + 8 * (int)threadIdx.x; f < n1; f += 2048)
                 *(u32x4_t*)(a.c + row * a.ldc_b + (size_t)f * 2) = *(const u32x4_t*)(a.r + row * a.ldr_b + (size_t)f * 2);
         }
         return;
-    }
-    // U of the tile as bf16 pairs in LDS: the workgroup's threads sum the slabs of four ranks each (loads of eight slabs in
-    // flight), ranks beyond the adapter's are zero
-    constexpr int UC = 32 * KS + 8;             // padded row: the fragment reads of 16 tokens fall on different banks
-    __shared__ __attribute__((aligned(16))) __bf16 us[2][16 * MT][UC];
-    const float s = a.scale ? a.scale[t.adapter] : 1.0f;
-    const size_t slab = (size_t)a.T * a.rank;
-    for (int e = threadIdx.x; e < 16 * MT * 8 * KS; e += 256) {
-        const int m = e / (8 * KS), r0 = 4 * (e % (8 * KS));
-        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-        if (r0 < a.rank) {
-            const float* up = a.u + (size_t)(t.s0 + min(t.t0 + m, t.n - 1)) * a.rank + r0;
-            for (int p = 0; p < a.ksplit; p += 8) {
-                f32x4_t w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = *(const f32x4_t*)(up + (size_t)min(p + i, a.ksplit - 1) * slab);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (p + i < a.ksplit) v += w[i];
-            }
-        }
-        bf16x4_t h4, l4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = s * v[j];
-            h4[j] = (__bf16)x;
-            l4[j] = (__bf16)(x - (float)h4[j]);
-        }
-        *(bf16x4_t*)&us[0][m][r0] = h4;
-        *(bf16x4_t*)&us[1][m][r0] = l4;
     }
     const char* bp = a.b + (size_t)t.adapter * a.N * a.rank * 2;
     // Steps of 256 features, 64 a wave.  R comes in and C goes out as contiguous 512 bytes of a row; the products meet them in an fp32
@@ -197,9 +170,39 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i)
-            rr[i] = *(const u32x4_t*)(a.r + (size_t)(t.s0 + min(t.t0 + 8 * i + lr, t.n - 1)) * a.ldr_b + (size_t)min(f0 + 8 * lc, a.N - 8) * 2);
+            rr[i] = *(const u32x4_t*)(a.r + (size_t)(t.row0 + min(8 * i + lr, t.n - 1)) * a.ldr_b + (size_t)min(f0 + 8 * lc, a.N - 8) * 2);
     };
     load(n0);                                   // flies while U is put together
+    // U of the tile as bf16 pairs in LDS: the workgroup's threads sum the slabs of four ranks each (loads of eight slabs in
+    // flight), ranks beyond the adapter's are zero
+    constexpr int UC = 32 * KS + 8;             // padded row: the fragment reads of 16 tokens fall on different banks
+    __shared__ __attribute__((aligned(16))) __bf16 us[2][16 * MT][UC];
+    const float s = a.scale ? a.scale[t.adapter] : 1.0f;
+    const size_t slab = (size_t)a.T * a.rank;
+    for (int e = threadIdx.x; e < 16 * MT * 8 * KS; e += 256) {
+        const int m = e / (8 * KS), r0 = 4 * (e % (8 * KS));
+        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+        if (r0 < a.rank) {
+            const float* up = a.u + (size_t)(t.row0 + min(m, t.n - 1)) * a.rank + r0;
+            for (int p = 0; p < a.ksplit; p += 8) {
+                f32x4_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = *(const f32x4_t*)(up + (size_t)min(p + i, a.ksplit - 1) * slab);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (p + i < a.ksplit) v += w[i];
+            }
+        }
+        bf16x4_t h4, l4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = s * v[j];
+            h4[j] = (__bf16)x;
+            l4[j] = (__bf16)(x - (float)h4[j]);
+        }
+        *(bf16x4_t*)&us[0][m][r0] = h4;
+        *(bf16x4_t*)&us[1][m][r0] = l4;
+    }
     __syncthreads();
     bf16x8_t hi[MT][KS], lo[MT][KS];            // U^T fragments: lane -> token col, ranks 32 k + 8 quad .. + 7
 #pragma unroll
@@ -238,43 +241,49 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
         if (f0 + 256 < n1) load(f0 + 256);
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) {
-            const int tok = t.t0 + 8 * i + lr;
-            if (tok < t.n && f0 + 8 * lc < n1) *(u32x4_t*)(a.c + (size_t)(t.s0 + tok) * a.ldc_b + (size_t)(f0 + 8 * lc) * 2) = out[i];
+            const int tok = 8 * i + lr;
+            if (tok < t.n && f0 + 8 * lc < n1) *(u32x4_t*)(a.c + (size_t)(t.row0 + tok) * a.ldc_b + (size_t)(f0 + 8 * lc) * 2) = out[i];
         }
         __syncthreads();
     }
 }
 
 struct Plan {
-    int mt, ksplit, kchunk, nslice;
+    int mt, ksplit, kchunk, nslice;             // mt: 16-token blocks per tile
     long long nslots;
 };
 
 Plan make_plan(int T, int B, int N, int K, int rank, int cus) {
     Plan p;
-    // 16 tokens a tile where sequences have no more on average, else 32: 64 measured slower (prompts of up to 1024 tokens, rank 32,
-    // 2048 -> 6144: 113 us with 32, 128 with 64, 124 with 16: fewer workgroups fit a CU)
+    // 16 tokens a tile where sequences have no more on average, else 32.  64 measured no faster in the first launch (24 us against 22, 17 k
+    // tokens, rank 32, 2048 -> 6144) and slower in the second (120 against 96: fewer workgroups fit a CU), 16 slower in both
     p.mt = (double)T / B <= 16 ? 1 : 2;
     p.nslots = (long long)T / (16 * p.mt) + B;
     const long long tiles = ((long long)T + 16 * p.mt - 1) / (16 * p.mt) > B ? ((long long)T + 16 * p.mt - 1) / (16 * p.mt) : B;
-    // K ranges: one workgroup per CU (every slab is read again by every slice of the second launch: 32 blocks of 32 tokens, rank 64,
-    // 6144 -> 2048 took 22.4 us so, 27.6 with two per CU), no range under one step of the four waves
-    long long ks = (cus + tiles - 1) / tiles;
+    // features of a workgroup: two steps where that leaves a workgroup per CU (U is put together once for both: 135 us against 143 on the
+    // same prompts, and four steps 138), else one
+    p.nslice = tiles * ((N + 511) / 512) >= cus ? 512 : 256;
+    // K ranges: one workgroup per CU; up to four where the slabs of U, written once and read by every slice of the second launch, stay under
+    // an eighth of X, R and C (prompts as above: 25 -> 22 us with two ranges; 32 blocks of 32 tokens, rank 64, 6144 -> 2048: 22.4 us with the
+    // eight ranges of one workgroup per CU, 27.6 with sixteen).  No range under one step of the four waves.
+    const long long slab = 4LL * rank * (1 + (N + p.nslice - 1) / p.nslice), most = (2LL * K + 4LL * N) / 8 / slab;
+    long long ks = (4LL * cus + tiles - 1) / tiles;
+    if (ks > most) ks = most;
+    if (ks < (cus + tiles - 1) / tiles) ks = (cus + tiles - 1) / tiles;
     if (ks > K / 256) ks = K / 256;
     if (ks < 1) ks = 1;
     p.kchunk = (int)(((K + ks - 1) / ks + 63) / 64 * 64);
     p.ksplit = (K + p.kchunk - 1) / p.kchunk;
-    // features of a workgroup: two steps where that leaves a workgroup per CU (U is put together once for both: 135 us against 143 on the
-    // prompts above, and four steps 138), else one
-    p.nslice = tiles * ((N + 511) / 512) >= cus ? 512 : 256;
     return p;
 }
+
+long long plan_bytes(const Plan& p, int T, int rank) { return p.nslots * (long long)sizeof(Tile) + (long long)p.ksplit * T * rank * 4; }
 
 }  // namespace
 
 extern "C" long long coda_lora_workspace_bytes(int T, int B, int N, int K, int rank) {
     if (T <= 0 || B <= 0 || N <= 0 || K <= 0 || rank <= 0) return 0;
-    return (long long)make_plan(T, B, N, K, rank, coda_device_cus()).ksplit * T * rank * 4;
+    return plan_bytes(make_plan(T, B, N, K, rank, coda_device_cus()), T, rank);
 }
 
 extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const void* Bw, const float* scale, const int* seq_start,
@@ -289,7 +298,7 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
     if (((uintptr_t)X | (uintptr_t)A | (uintptr_t)Bw | (uintptr_t)R | (uintptr_t)C) & 15 || (ldx * 2) % 16 || (ldr * 2) % 16 || (ldc * 2) % 16)
         return coda_refuse(who, CODA_ERR_ALIGN, "rows start on 16 bytes");
     const Plan p = make_plan(T, B, N, K, rank, coda_device_cus());
-    if (!workspace || workspace_bytes < (long long)p.ksplit * T * rank * 4)
+    if (!workspace || workspace_bytes < plan_bytes(p, T, rank))
         return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_lora_workspace_bytes");
     if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
     const long long downs = p.nslots * p.ksplit, ups = p.nslots * ((N + p.nslice - 1) / p.nslice);
@@ -302,7 +311,8 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
     a.c = (char*)C; a.ldc_b = ldc * 2;
     a.N = N; a.K = K;
     a.nslots = (int)p.nslots; a.ksplit = p.ksplit; a.kchunk = p.kchunk; a.nslice = p.nslice;
-    a.u = (float*)workspace;
+    a.tiles = (Tile*)workspace;
+    a.u = (float*)(a.tiles + p.nslots);
     hipStream_t st = (hipStream_t)stream;
     const dim3 gd((unsigned)downs), gu((unsigned)ups), block(256);
     auto down = [&](auto kernel, int lds) -> int {
