@@ -45,7 +45,8 @@ struct AttnArgs {
     int* range_keys;                           // the range length that the first kernel took, for the second
 };
 
-__device__ __forceinline__ int swz(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+// row bits 0..3 to the 16 chunk positions; the low two so that the transposing reads of 16 keys (few rows) fall on different banks too
+__device__ __forceinline__ int swz(int row) { return ((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1); }
 
 typedef __attribute__((ext_vector_type(8))) short s16x8_t;
 
@@ -58,7 +59,7 @@ struct TileRows {
 };
 
 struct Limits {
-    int kv; long long pos0;
+    int kv, pos0;
 };
 
 __device__ __forceinline__ int kv_of(const AttnArgs& a, int x) { return min(max(x, 0), a.max_kv); }
@@ -100,17 +101,20 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, TileRows&
         const int kv = kv_of(a, l.x);
         return tiles_of<R>(l, a.g) * (a.max_ranges > 1 ? max(1, (kv + range_keys - 1) / range_keys) : 1);
     });
-    if (q.b < 0) return false;
+    if (__builtin_amdgcn_readfirstlane(q.b) < 0) return false;
     lm = limits_of(a, q);
     const int rows = q.n * a.g, tiles = rows / R + (rows % R != 0), ranges = max(1, (lm.kv + range_keys - 1) / range_keys);
-    // later tiles see more keys under a mask: they go first
-    t = {q.b, q.s0, q.n, (tiles - 1 - k / ranges) * R, rows, k % ranges, keys_of(lm.kv, range_keys)};
+    // Later tiles see more keys under a mask: they go first.  All of this is the same in every lane, which the compiler does not find out
+    // by itself (loops, ballots): told so, it keeps what follows from it - bounds, page bases, branches - in scalar registers.
+    auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    t = {u(q.b), u(q.s0), u(q.n), u((tiles - 1 - k / ranges) * R), u(rows), u(k % ranges), u(keys_of(lm.kv, range_keys))};
+    lm = {u(lm.kv), u(lm.pos0)};
     return true;
 }
 
 __device__ __forceinline__ int limit_of(const AttnArgs& a, const Limits& l, int token) {
     if (a.mask_block == 0) return l.kv;
-    const long long p = l.pos0 + token;
+    const long long p = (long long)l.pos0 + token;
     if (p < 0) return 0;
     const long long end = ((long long)((unsigned int)p / (unsigned int)a.mask_block) + 1) * a.mask_block;
     return (int)min((long long)l.kv, end);
@@ -138,57 +142,57 @@ __device__ __forceinline__ size_t shfl_size(size_t v, int src) {
     return ((size_t)hi << 32) | lo;
 }
 
-// Source addresses of a tile's 1 KiB pieces (4 bf16 or 8 e4m3 keys each).  Pages of a multiple of 16 keys (G16): any 16 aligned
-// keys lie on one page, one after the other, so a group of 16 has ONE wave-uniform base, its pieces are whole contiguous KiB at
-// constant offsets from it and the address costs no vector instruction.  Other page sizes: lane l looks key l of the tile up and the
-// loads fetch their key's offset from it by shuffles.
-// A wave fetches pieces first, first + STRIDE, ... (NP of them).
-template <int KEYS, int NP, int STRIDE, bool F8, bool G16>
-struct TileSource {
-    static constexpr int GROUPS = KEYS / 16;
-    static constexpr int PROWS = F8 ? 8 : 4;
-    static constexpr int SUB = F8 ? 8 : 16;    // lanes per key
-    int first;
-    size_t base[G16 ? NP : 1];                 // G16: of each piece's group (uniform); else: of key lane & (KEYS - 1)
-    unsigned long long ok;                     // keys that exist
-    int entry;                                 // page number of the tile looked up last, lane l: of group l (G16) or key l
+// Where the keys of a range are, looked up ahead.
+// Pages of a multiple of 16 keys (G16): 16 aligned keys lie on one page, one after the other.  Lane l holds the offset of 16-key group
+// 64 w + l of window w (1024 keys), so a tile's groups come out by readlane as wave-uniform bases, their keys are whole contiguous
+// KiB at constant offsets from them, and most tiles cost no look-up at all.
+// Other page sizes: lane l holds the offset of key l of the tile.
+template <int KEYS, bool G16>
+struct PageSource {
+    static constexpr int UNIT = G16 ? 16 : 1, SPAN = G16 ? 64 : KEYS;     // keys per lane, lanes per look-up
+    unsigned int lo, hi;                       // offset inside the cache
+    unsigned long long there;                  // lanes whose page exists
+    int entry;                                 // page number of the next look-up, on its way
+    int at;                                    // next look-up (window or tile)
 
-    // a vector load also where all lanes want few numbers: a scalar one would be waited for with the next LDS read, a tile early
-    __device__ __forceinline__ void look_up(const AttnArgs& a, const int* table, int key0, int end) {
-        const int lane = threadIdx.x & 63;
-        entry = page_entry(a, table, key0 + (G16 ? 16 * (lane & (GROUPS - 1)) : lane & (KEYS - 1)), end);
+    __device__ __forceinline__ int key_of(int w) const { return (w * SPAN + (int)(threadIdx.x & (SPAN - 1))) * UNIT; }
+    // `first`: tile
+    __device__ __forceinline__ void start(const AttnArgs& a, const int* table, int k_lo, int k_hi, int first) {
+        at = G16 ? first * (KEYS / 16) / 64 : first;
+        entry = page_entry(a, table, k_lo + key_of(at), k_hi);
     }
-    // page numbers -> offsets, for the tile that look_up was last called for
-    __device__ __forceinline__ void resolve(const AttnArgs& a, int key0, int end) {
-        const int lane = threadIdx.x & 63;
-        if (G16) {
-            const int key = key0 + 16 * (lane & (GROUPS - 1));
-            const KeyAt at = key_at(a, entry, key);
-            ok = 0;
+    // makes tile t's keys known and sends for what a later one needs (G16: the next window; else the tile after t by `step`)
+    __device__ __forceinline__ void advance(const AttnArgs& a, const int* table, int k_lo, int k_hi, int t, int step) {
+        if (G16 && t * (KEYS / 16) / 64 != at) return;          // still the window before
+        const KeyAt k = key_at(a, entry, k_lo + key_of(at));
+        lo = (unsigned)k.off;
+        hi = (unsigned)(k.off >> 32);
+        there = __ballot(k.ok);
+        at += G16 ? 1 : step;
+        entry = page_entry(a, table, k_lo + key_of(at), k_hi);
+    }
+    // keys of tile t that exist, lowest bit first
+    __device__ __forceinline__ unsigned long long exist(int k_lo, int k_hi, int t) const {
+        constexpr unsigned long long ALL = KEYS == 64 ? ~0ull : (1ull << (KEYS & 63)) - 1;
+        if (!G16) return there & ALL;
+        constexpr int G = KEYS / 16;
+        const unsigned int g = (unsigned int)(there >> (t * G & 63)) & ((1u << G) - 1);
+        if (g == (1u << G) - 1 && k_lo + (t + 1) * KEYS <= k_hi) return ALL;
+        unsigned long long ok = 0;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const int live = __builtin_amdgcn_readlane((int)at.ok, g) ? min(max(end - key0 - 16 * g, 0), 16) : 0;
-                ok |= (unsigned long long)((1u << live) - 1u) << (16 * g);
-            }
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int g = (i * STRIDE + first) * PROWS / 16;
-                const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)at.off, g), hi = __builtin_amdgcn_readlane((int)(unsigned)(at.off >> 32), g);
-                base[i] = ((size_t)hi << 32) | lo;
-            }
-        } else {
-            const KeyAt at = key_at(a, entry, key0 + (lane & (KEYS - 1)));
-            ok = __ballot(at.ok);
-            if (KEYS < 64) ok &= (1ull << (KEYS & 63)) - 1;
-            base[0] = at.off;
+        for (int i = 0; i < G; ++i) {
+            const int live = (g >> i) & 1 ? min(max(k_hi - k_lo - t * KEYS - 16 * i, 0), 16) : 0;
+            ok |= (unsigned long long)((1u << live) - 1u) << (16 * i);
         }
+        return ok;
     }
-    // this lane's 16 bytes of the wave's piece i
-    __device__ __forceinline__ size_t at(int i) const {
-        const int lane = threadIdx.x & 63, key = (i * STRIDE + first) * PROWS;
-        if (G16) return base[i] + (size_t)((key & 15) * (16 * SUB) + lane * 16);
-        return shfl_size(base[0], key + lane / SUB) + (lane % SUB) * 16;
+    // G16: uniform offset of group i of tile t
+    __device__ __forceinline__ size_t group(int t, int i) const {
+        const int l = (t * (KEYS / 16) + i) & 63;
+        return ((size_t)(unsigned)__builtin_amdgcn_readlane((int)hi, l) << 32) | (unsigned)__builtin_amdgcn_readlane((int)lo, l);
     }
+    // else: offset of key i (per lane)
+    __device__ __forceinline__ size_t key(int i) const { return shfl_size(((size_t)hi << 32) | lo, i); }
 };
 
 // four e4m3 bytes -> four bf16 (exact: three mantissa bits, exponents within bf16's)
@@ -216,11 +220,11 @@ __device__ __forceinline__ bool drop_nonfinite(u32x4_t& v) {
 
 // A tile that some row sees only in part holds values of keys that other rows must not feel, and the products cannot skip
 // them: 0 * inf = NaN.  Staging such a tile drops its infinities and NaN from the LDS image; if there were any, this finds
-// the outputs they belong to: those features of the rows that do see their key come out as NaN.  Bit 16 db + i of the answer
-// stands for accumulator register i of feature block db.  Rare, and slow on purpose: a rolled loop that needs no registers.
-template <bool F8>
+// the outputs they belong to: those features of the rows that do see their key come out as NaN.  Bit e of the answer stands for
+// feature feature(e), e < n.  Rare, and slow on purpose: a rolled loop that needs no registers.
+template <bool F8, class F>
 __device__ __forceinline__ unsigned long long find_nonfinite(const AttnArgs& a, const int* table, size_t head_off, int key0, int nkeys,
-                                                             int end, int lim, int half) {
+                                                             int end, int lim, int n, F feature) {
     unsigned long long bits = 0;
 #pragma unroll 1
     for (int j = 0; j < nkeys; ++j) {
@@ -229,22 +233,13 @@ __device__ __forceinline__ unsigned long long find_nonfinite(const AttnArgs& a, 
         if (key >= end || !at.ok || key >= lim) continue;
         const char* p = a.v + head_off + at.off;
 #pragma unroll 1
-        for (int e = 0; e < 64; ++e) {
-            const int d = 32 * (e >> 4) + (e & 3) + 8 * ((e >> 2) & 3) + 4 * half;
+        for (int e = 0; e < n; ++e) {
+            const int d = feature(e);
             const bool bad = F8 ? (((const unsigned char*)p)[d] & 0x7f) == 0x7f : (((const unsigned short*)p)[d] & 0x7f80) == 0x7f80;
             if (bad) bits |= 1ull << e;
         }
     }
     return bits;
-}
-
-__device__ __forceinline__ void poison(f32x16_t (&o)[4], unsigned long long bits) {
-    if (!__any(bits != 0)) return;
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if ((bits >> (16 * db + i)) & 1) o[db][i] = __builtin_nanf("");
 }
 
 // output row of a tile row: token row and head
@@ -265,102 +260,88 @@ __device__ __forceinline__ u32x4_t pack8(const float (&f)[8]) {
     return v;
 }
 
-// Writes a lane's 16 bytes of a K and of a V piece into the tile images (bf16 rows of 256 B, chunk ch of key r at ch ^ swz(r)).
-// PART: keys that do not exist become zeros in the V image, and so do infinities and NaN; true if there were any of those.
+// weight of a part with maximum m in a sum with maximum mm; a part without a maximum holds zeros (or NaN): nothing to scale
+__device__ __forceinline__ float part_weight(float m, float mm) { return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mm); }
+
+// Writes a lane's 16 bytes of a K or V piece (4 bf16 or 8 e4m3 keys) into a tile image: bf16 rows of 256 B, chunk ch of key r at
+// ch ^ swz(r).  PART (V images): keys that do not exist become zeros, and so do infinities and NaN; true if there were any of those.
 template <bool F8>
 struct ImageWriter {
     int row0, at0;                             // key within the piece, and its byte offset with the swizzle's lane-dependent part
     __device__ __forceinline__ explicit ImageWriter(int lane) {
         row0 = F8 ? lane >> 3 : lane >> 4;
         const int ch = F8 ? 2 * (lane & 7) : lane & 15;
-        at0 = row0 * 256 + ((ch ^ ((row0 & 3) << 2)) << 4);
+        at0 = row0 * 256 + ((ch ^ swz(row0)) << 4);
     }
     template <bool PART>
-    __device__ __forceinline__ bool put(char* kimg, char* vimg, int piece, const u32x4_t& k, const u32x4_t& v, unsigned long long ok) const {
+    __device__ __forceinline__ bool put(char* img, int piece, const u32x4_t& v, unsigned long long ok) const {
         bool dropped = false;
         const bool live = !PART || ((ok >> (piece * (F8 ? 8 : 4) + row0)) & 1);
         const u32x4_t zero = {0, 0, 0, 0};
+        // swz(a + b) = swz(a) ^ swz(b) for parts without common bits
         if (F8) {
-            // key 8 piece + row0: swz's low part is (2 piece + (row0 >> 2)) & 3
-            const int x = (((2 * piece) & 3) ^ (row0 >> 2)) << 4;
+            const int at = piece * 2048 + (at0 ^ (swz(8 * (piece & 1)) << 4));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const u32x2_t k0 = bf16_of_e4m3(k[2 * j]), k1 = bf16_of_e4m3(k[2 * j + 1]);
                 const u32x2_t v0 = bf16_of_e4m3(v[2 * j]), v1 = bf16_of_e4m3(v[2 * j + 1]);
-                u32x4_t vw = {v0[0], v0[1], v1[0], v1[1]};
+                u32x4_t w = {v0[0], v0[1], v1[0], v1[1]};
                 if (PART) {
-                    if (!live) vw = zero;
-                    dropped |= drop_nonfinite(vw);
+                    if (!live) w = zero;
+                    dropped |= drop_nonfinite(w);
                 }
-                const int at = piece * 2048 + (at0 ^ x ^ (j << 4));
-                *(u32x4_t*)(kimg + at) = (u32x4_t){k0[0], k0[1], k1[0], k1[1]};
-                *(u32x4_t*)(vimg + at) = vw;
+                *(u32x4_t*)(img + (at ^ (j << 4))) = w;
             }
         } else {
-            // key 4 piece + row0: swz's low part is piece & 3
-            u32x4_t vw = v;
+            u32x4_t w = v;
             if (PART) {
-                if (!live) vw = zero;
-                dropped = drop_nonfinite(vw);
+                if (!live) w = zero;
+                dropped = drop_nonfinite(w);
             }
-            const int at = piece * 1024 + (at0 ^ ((piece & 3) << 4));
-            *(u32x4_t*)(kimg + at) = k;
-            *(u32x4_t*)(vimg + at) = vw;
+            *(u32x4_t*)(img + piece * 1024 + (at0 ^ (swz(4 * (piece & 3)) << 4))) = w;
         }
         return dropped;
     }
 };
 
-// MFMA fragments out of the images.
-//   K (A operand of S^T, 32 keys x 16 features): lane -> key 32 k2 + (lane & 31), chunk 2 ks + (lane >> 5)
-//   V^T (A operand of O^T, 32 features x 16 keys): the transposing read; lane i16 = lane & 15 addresses key tq = i16 >> 2 of
-//   the quad 16 st + 4 h (and + 8), chunk 4 db + 2 ((lane >> 4) & 1) + ((i16 & 3) >> 1), byte 8 (i16 & 1)
-// The offsets are recomputed from two registers per tile instead of being kept in a dozen (the empty asm hides that they do not
-// change): an exclusive-or per read is free next to the matrix instructions, the registers are not.
-struct ImageReader {
-    int k0, v0;
-    __device__ __forceinline__ explicit ImageReader(int lane) {
-        const int c = lane & 31, h = lane >> 5;
-        k0 = c * 256 + ((h ^ swz(c)) << 4);
-        const int i16 = lane & 15, tq = i16 >> 2, tp = i16 & 3;
-        const int ch = 2 * ((lane >> 4) & 1) + (tp >> 1);
-        v0 = (4 * h + tq) * 256 + ((ch ^ ((tq << 2) | h)) << 4) + 8 * (tp & 1);
-    }
-    __device__ __forceinline__ bf16x8_t k(const char* img, int k2, int ks) const {
-        return *(const bf16x8_t*)(img + 32 * k2 * 256 + (k0 ^ (ks << 5)));
-    }
-    __device__ __forceinline__ bf16x8_t v(const char* img, int st, int db) const {
-        // key quads 16 st + 4 h and 16 st + 4 h + 8: swz differs in bit 1 (chunk ^ 2)
-        const char* p = img + st * 4096;
-        const int at = v0 ^ (db << 6);
-        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CODA_LDS s16x4_t*)(p + at));
-        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CODA_LDS s16x4_t*)(p + 2048 + (at ^ 32)));
-        const s16x8_t v8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        return __builtin_bit_cast(bf16x8_t, v8);
-    }
-};
+// four keys x 16 features, transposed on the way: lane i of a group of 16 addresses 8 bytes (key i >> 2, features 4 (i & 3) ..) and
+// receives feature i of the four keys
+__device__ __forceinline__ s16x4_t read_transposed(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((CODA_LDS s16x4_t*)p); }
+
+__device__ __forceinline__ bf16x8_t join4(s16x4_t a, s16x4_t b) {
+    const s16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return __builtin_bit_cast(bf16x8_t, v);
+}
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few rows (RG groups of 32 per tile): the four waves of a workgroup take KEY tiles in turn, each with its own LDS image, maximum, sum and
-// output; they meet once, at the end.  No barrier in the loop.
+// Few rows: RW x RG groups of 16.  Four KEY waves per row wave take tiles of 32 keys in turn, each with its own V image, maximum, sum
+// and output; they meet once, at the end.  No barrier in the loop.
+//
+// What bounds it: the bytes of the cache (decode), or the latency of one tile after the other (short sequences).  So the next tile's
+// pages are in flight under this one's products, K goes from memory straight into the A fragments of v_mfma_f32_16x16x32_bf16 (a
+// quarter-wave reads 64 B of a key, the fragments of a tile are whole lines) and only V passes LDS, for its transposition.
+//   S^T[key][row]:  lane -> row lane & 15, keys 16 kt + 4 quad + i          (quad = lane >> 4)
+//   P^T as B:       k index (quad, j) is key 16 (j >> 2) + 4 quad + (j & 3): the accumulators as they are
+//   O^T[d][row]:    lane -> row lane & 15, features 16 dt + 4 quad + i
 constexpr int FEW_TILE = 32;                                    // keys per tile
-constexpr int FEW_WAVE_LDS = 2 * FEW_TILE * 256;                // K and V image: 16 KiB a wave
+constexpr int FEW_WAVE_LDS = FEW_TILE * 256;                    // V image, then 16 rows of fp32 output: 8 KiB a wave
 
-template <int RG, bool F8, bool G16>
-__global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(AttnArgs a) {
+template <int RG, int RW, bool F8, bool G16>
+__global__ __launch_bounds__(256 * RW, RG == 1 && F8 ? 3 : 2) void paged_attn_few_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int R = 32 * RG;
-    constexpr int NP = F8 ? 4 : 8;                              // 1 KiB pieces of a K (or V) tile
-    __shared__ float ml[4][2][R];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 31, h = lane >> 5;
+    constexpr int R = 16 * RG * RW;
+    constexpr int NP = F8 ? 4 : 8;                              // 1 KiB pieces of a K or V tile
+    // weights as a bf16 pair (value and remainder): the second product per fragment hides under the page loads, and the weights keep
+    // 16 significant bits instead of 8
+    __shared__ float ml[4 * RW][2][16 * RG];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = wave & 3, rw = wave >> 2;
+    const int c = lane & 15, quad = lane >> 4;
     const int kvh = blockIdx.x % a.n_kv;
     TileRows tr;
     Limits lm;
     if (!find_unit<R>(a, blockIdx.x / a.n_kv, tr, lm)) return;
     const int last = min(tr.r0 + R, tr.rows) - 1;               // last live row of the tile
-    const int end = limit_of(a, lm, fast_div(a.gdiv, last));    // keys that any row of the tile sees
-    const int all = limit_of(a, lm, fast_div(a.gdiv, tr.r0));   // keys that every row of it sees
+    const int end = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, last)));    // keys that any row of the tile sees
+    const int all = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, tr.r0)));   // keys that every row of it sees
     const int nsp = a.max_ranges > 1 ? max(1, (end + tr.keys - 1) / tr.keys) : 1;
     if (tr.range >= nsp) return;
     const int k_lo = tr.range * tr.keys, k_hi = min(end, k_lo + tr.keys);
@@ -368,78 +349,112 @@ __global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(At
     const int* table = a.pg.table + (size_t)tr.b * a.pg.ld_table;
     const char* kbase = a.k + head_off;
     const char* vbase = a.v + head_off;
+    const int nt = (k_hi - k_lo + FEW_TILE - 1) / FEW_TILE;     // may be <= 0: rows that see no key
 
-    bf16x8_t qf[RG][8];
+    PageSource<FEW_TILE, G16> src;
+    u32x4_t kr[NP], vr[NP];
+    unsigned int ok = 0;                                        // keys of the fetched tile that exist
+    auto fetch = [&](int t) {
+        src.advance(a, table, k_lo, k_hi, t, 4);
+        ok = (unsigned int)src.exist(k_lo, k_hi, t);
+        constexpr int ROW = F8 ? 128 : 256, PROWS = F8 ? 8 : 4, SUB = F8 ? 8 : 16;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {                           // K: a lane's key of each half of the tile, 64 B of 16 keys a piece
+            const size_t at = G16 ? src.group(t, g) : src.key(16 * g + c);
+            const char* p = kbase + at;
+            const unsigned int in = (G16 ? c * ROW : 0) + quad * 16;
+#pragma unroll
+            for (int ks = 0; ks < NP / 2; ++ks) kr[g * (NP / 2) + ks] = *(const u32x4_t*)(p + in + ks * 64);
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {                          // V: whole KiB, 64 / SUB keys
+            const char* p = vbase + (G16 ? src.group(t, i * PROWS / 16) : src.key(i * PROWS + lane / SUB));
+            const unsigned int in = G16 ? i * PROWS % 16 * ROW + lane * 16 : (lane % SUB) * 16;
+            vr[i] = *(const u32x4_t*)(p + in);
+        }
+    };
+    if (kw < nt) {
+        src.start(a, table, k_lo, k_hi, kw);
+        fetch(kw);
+    }
+
+    // ---- queries: lane -> row c, features as the K fragments have them
+    bf16x8_t qf[RG][4];
     int lim[RG];
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-        const int r = min(tr.r0 + rg * 32 + c, tr.rows - 1);
-        const RowAt at = row_at(a, tr, kvh, r);
+        const RowAt at = row_at(a, tr, kvh, min(tr.r0 + (rw * RG + rg) * 16 + c, tr.rows - 1));
         lim[rg] = limit_of(a, lm, at.token - tr.s0);
-        const char* qp = a.q + (size_t)at.token * a.ldq_b + (size_t)at.head * 256 + h * 16;
+        const char* qp = a.q + (size_t)at.token * a.ldq_b + (size_t)at.head * 256;
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) qf[rg][ks] = *(const bf16x8_t*)(qp + ks * 32);
+        for (int ks = 0; ks < 4; ++ks) qf[rg][ks] = *(const bf16x8_t*)(qp + (F8 ? 8 * (ks >> 1) + 2 * quad + (ks & 1) : 4 * ks + quad) * 16);
     }
 
-    char* kimg = lds + wave * FEW_WAVE_LDS;
-    char* vimg = kimg + FEW_TILE * 256;
-    f32x16_t o[RG][4];
+    char* vimg = lds + wave * FEW_WAVE_LDS;
+    f32x4_t o[RG][8];
     float m_run[RG], l_run[RG];
-    unsigned long long bad[RG];
+    unsigned int bad[RG];
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
 #pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[rg][db][i] = 0.f;
+        for (int dt = 0; dt < 8; ++dt) o[rg][dt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
         m_run[rg] = -INFINITY;
         l_run[rg] = 0.f;
         bad[rg] = 0;
     }
+    const ImageWriter<F8> img(lane);
+    // V^T fragments: keys 4 quad .. + 3 and 16 + 4 quad .. + 3, features 16 dt + c
+    const int v0 = (4 * quad + (c >> 2)) * 256 + ((((c >> 1) & 1) ^ swz(4 * quad + (c >> 2))) << 4) + 8 * (c & 1);
 
-    u32x4_t kr[NP], vr[NP];
-    TileSource<FEW_TILE, NP, 1, F8, G16> src;
-    src.first = 0;
-    auto fetch = [&] {
+    for (int t = kw; t < nt; t += 4) {
+        const unsigned int ok_t = ok;
+        const int key0 = k_lo + t * FEW_TILE;
+        const bool part = ok_t != 0xffffffffu || key0 + FEW_TILE > all;           // wave-uniform
+        bool dropped = false;
+        // ---- S^T
+        f32x4_t s[RG][2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) s[rg][g] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                bf16x8_t kf;
+                if (F8) {
+                    const u32x4_t w = kr[2 * g + (ks >> 1)];
+                    const u32x2_t x = bf16_of_e4m3(w[2 * (ks & 1)]), y = bf16_of_e4m3(w[2 * (ks & 1) + 1]);
+                    kf = __builtin_bit_cast(bf16x8_t, (u32x4_t){x[0], x[1], y[0], y[1]});
+                } else {
+                    kf = __builtin_bit_cast(bf16x8_t, kr[(4 * g + ks) % NP]);
+                }
+#pragma unroll
+                for (int rg = 0; rg < RG; ++rg) s[rg][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rg][ks], s[rg][g], 0, 0, 0);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const size_t off = src.at(i);
-            kr[i] = *(const u32x4_t*)(kbase + off);
-            vr[i] = *(const u32x4_t*)(vbase + off);
-            if (!G16 && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // bounds the addresses alive at once
+            if (part) dropped |= img.template put<true>(vimg, i, vr[i], ok_t);
+            else img.template put<false>(vimg, i, vr[i], ok_t);
         }
-    };
-    const ImageWriter<F8> img(lane);
-    const ImageReader rd(lane);
-
-    auto tile = [&](int t, bool part, bool dropped, unsigned int ok) {
-        const int key0 = k_lo + t * FEW_TILE;
-        f32x16_t s[RG];
-#pragma unroll
-        for (int rg = 0; rg < RG; ++rg)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[rg][i] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-            const bf16x8_t kf = rd.k(kimg, 0, ks);
-#pragma unroll
-            for (int rg = 0; rg < RG; ++rg) s[rg] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[rg][ks], s[rg], 0, 0, 0);
-        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + 4 < nt) fetch(t + 4);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int rg = 0; rg < RG; ++rg) {
             if (part) {                                         // uniform, and kept a branch by the empty asm
                 asm volatile("" ::: "memory");
-                const int left = lim[rg] - key0 - 4 * h;
-                const unsigned int okh = ok >> (4 * h);
+                const int left = lim[rg] - key0 - 4 * quad;
+                const unsigned int okq = ok_t >> (4 * quad);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = (i & 3) + 8 * (i >> 2);
-                    if (j >= left || !((okh >> j) & 1)) s[rg][i] = -INFINITY;
-                }
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * g + i >= left || !((okq >> (16 * g + i)) & 1)) s[rg][g][i] = -INFINITY;
             }
-            float mx = s[rg][0];
+            float mx = fmaxf(s[rg][0][0], s[rg][1][0]);
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[rg][i]);
+            for (int i = 1; i < 4; ++i) mx = fmaxf(mx, fmaxf(s[rg][0][i], s[rg][1][i]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
             if (__any(mx > m_run[rg] + RESCALE_THR)) {
                 const float m_new = fmaxf(m_run[rg], mx);
@@ -448,124 +463,89 @@ __global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(At
                 l_run[rg] *= alpha;
                 m_run[rg] = m_new;
 #pragma unroll
-                for (int db = 0; db < 4; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[rg][db][i] *= alpha;
+                for (int dt = 0; dt < 8; ++dt) o[rg][dt] *= alpha;
             }
             const float neg_m = m_run[rg] == -INFINITY ? 0.f : -m_run[rg];
             float psum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rg][i], a.scale_log2e, neg_m));
-                s[rg][i] = p;
-                psum += p;
-            }
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rg][g][i], a.scale_log2e, neg_m));
+                    s[rg][g][i] = p;
+                    psum += p;
+                }
             l_run[rg] += psum;
         }
+        // ---- O^T
+        bf16x8_t ph[RG], pl[RG];
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-            bf16x8_t ph[RG], pl[RG];
-            // weights as a bf16 pair (value and remainder): the second product per fragment hides under the page loads, and
-            // the weights keep 16 significant bits instead of 8
+        for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = s[rg][j >> 2][j & 3];
+                ph[rg][j] = (__bf16)p;
+                pl[rg][j] = (__bf16)(p - (float)ph[rg][j]);
+            }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            // rows + 16: the same swizzle; features 16 dt: chunk 2 dt
+            const bf16x8_t vf = join4(read_transposed(vimg + (v0 ^ (dt << 5))), read_transposed(vimg + 4096 + (v0 ^ (dt << 5))));
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) {
+                o[rg][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[rg], o[rg][dt], 0, 0, 0);
+                o[rg][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph[rg], o[rg][dt], 0, 0, 0);
+            }
+        }
+        if (__any(dropped)) {
 #pragma unroll
             for (int rg = 0; rg < RG; ++rg)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float p = s[rg][8 * st + j];
-                    ph[rg][j] = (__bf16)p;
-                    pl[rg][j] = (__bf16)(p - (float)ph[rg][j]);
-                }
-#pragma unroll
-            for (int db = 0; db < 4; ++db) {
-                const bf16x8_t vf = rd.v(vimg, st, db);
-#pragma unroll
-                for (int rg = 0; rg < RG; ++rg) {
-                    o[rg][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, ph[rg], o[rg][db], 0, 0, 0);
-                    o[rg][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pl[rg], o[rg][db], 0, 0, 0);
-                }
-            }
-        }
-        if (dropped) {
-#pragma unroll
-            for (int rg = 0; rg < RG; ++rg) bad[rg] |= find_nonfinite<F8>(a, table, head_off, key0, FEW_TILE, k_hi, lim[rg], h);
-        }
-    };
-
-    const int nt = (k_hi - k_lo + FEW_TILE - 1) / FEW_TILE;     // may be <= 0: rows that see no key
-    if (wave < nt) {
-        src.look_up(a, table, k_lo + wave * FEW_TILE, k_hi);
-        src.resolve(a, k_lo + wave * FEW_TILE, k_hi);
-        fetch();
-        src.look_up(a, table, k_lo + (wave + 4) * FEW_TILE, k_hi);
-        for (int t = wave; t < nt; t += 4) {
-            const unsigned int ok = (unsigned int)src.ok;
-            const bool part = ok != 0xffffffffu || k_lo + (t + 1) * FEW_TILE > all;      // wave-uniform
-            bool dropped = false;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                if (part) dropped |= img.template put<true>(kimg, vimg, i, kr[i], vr[i], ok);
-                else img.template put<false>(kimg, vimg, i, kr[i], vr[i], ok);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if (t + 4 < nt) {
-                src.resolve(a, k_lo + (t + 4) * FEW_TILE, k_hi);
-                fetch();
-                src.look_up(a, table, k_lo + (t + 8) * FEW_TILE, k_hi);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            tile(t, part, __any(dropped), ok);
+                bad[rg] |= (unsigned int)find_nonfinite<F8>(a, table, head_off, key0, FEW_TILE, k_hi, lim[rg], 32,
+                                                            [&](int e) { return 16 * (e >> 2) + 4 * quad + (e & 3); });
         }
     }
 
-    // ---- the four waves' triples: common maximum, scaled sums
-    float l_half[RG];
+    // ---- the four key waves' triples: common maximum, scaled sums
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-        poison(o[rg], bad[rg]);
-        l_half[rg] = l_run[rg] + __shfl_xor(l_run[rg], 32, 64);
-        if (h == 0) {
-            ml[wave][0][rg * 32 + c] = m_run[rg];
-            ml[wave][1][rg * 32 + c] = l_half[rg];
+        if (__any(bad[rg] != 0)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if ((bad[rg] >> e) & 1) o[rg][e >> 2][e & 3] = __builtin_nanf("");
+        }
+        float l = l_run[rg] + __shfl_xor(l_run[rg], 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (quad == 0) {
+            ml[wave][0][rg * 16 + c] = m_run[rg];
+            ml[wave][1][rg * 16 + c] = l;
         }
     }
     __syncthreads();
+    const int w0 = rw * 4;                                      // first of this row wave's four
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-        const int r = rg * 32 + c;
-        float m = ml[0][0][r];
+        float m = ml[w0][0][rg * 16 + c];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][0][r]);
-        // a wave without a maximum holds sums of 0, or NaN where every score it saw was NaN: nothing to scale
-        const float f = m_run[rg] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[rg] - m);
-        // a wave's own image region holds its 32 x 128 fp32 block: 16-byte chunk ch of row r at ch ^ r
-        char* ob = lds + wave * FEW_WAVE_LDS;
+        for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w0 + w][0][rg * 16 + c]);
+        const float f = part_weight(m_run[rg], m);
+        // a wave's own image region holds its 16 x 128 fp32 block: 16-byte chunk ch of row r at ch ^ r
         if (rg > 0) __syncthreads();                            // the block of the previous row group has been read
 #pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-                f32x4_t x;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = o[rg][db][4 * i4 + j] * f;
-                *(f32x4_t*)(ob + c * 512 + (((8 * db + 2 * i4 + h) ^ c) << 4)) = x;
-            }
+        for (int dt = 0; dt < 8; ++dt) *(f32x4_t*)(vimg + c * 512 + (((4 * dt + quad) ^ c) << 4)) = o[rg][dt] * f;
         __syncthreads();
-        // wave w joins rows 8 w .. 8 w + 7: lane -> row, 16 features
-        const int rr = wave * 8 + (lane >> 3), ch0 = (lane & 7) * 4;
-        const int tile_row = tr.r0 + rg * 32 + rr;
-        float acc[16];
+        // key wave w joins rows 4 w .. 4 w + 3: lane -> row, 8 features
+        const int rr = kw * 4 + quad, tile_row = tr.r0 + (rw * RG + rg) * 16 + rr;
+        float acc[8], ll = 0.f, mm = ml[w0][0][rg * 16 + rr];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-        float mm = ml[0][0][rg * 32 + rr], ll = 0.f;
+        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
 #pragma unroll
-        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, ml[w][0][rg * 32 + rr]);
+        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, ml[w0 + w][0][rg * 16 + rr]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float mw = ml[w][0][rg * 32 + rr];
-            ll += ml[w][1][rg * 32 + rr] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - mm));
+            ll += ml[w0 + w][1][rg * 16 + rr] * part_weight(ml[w0 + w][0][rg * 16 + rr], mm);
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                const f32x4_t x = *(const f32x4_t*)(lds + w * FEW_WAVE_LDS + rr * 512 + (((ch0 + q4) ^ rr) << 4));
+            for (int q4 = 0; q4 < 2; ++q4) {
+                const f32x4_t x = *(const f32x4_t*)(lds + (w0 + w) * FEW_WAVE_LDS + rr * 512 + (((2 * c + q4) ^ rr) << 4));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[4 * q4 + j] += x[j];
             }
@@ -574,20 +554,15 @@ __global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(At
         const RowAt at = row_at(a, tr, kvh, tile_row);
         if (nsp == 1) {
             const float inv = ll == 0.f ? 0.f : a.v_scale / ll;            // no key seen: zeros
-            char* op = a.out + (size_t)at.token * a.ldo_b + (size_t)at.head * 256 + ch0 * 8;
 #pragma unroll
-            for (int q8 = 0; q8 < 2; ++q8) {
-                float y[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = acc[8 * q8 + j] * inv;
-                *(u32x4_t*)(op + q8 * 16) = pack8(y);
-            }
+            for (int j = 0; j < 8; ++j) acc[j] *= inv;
+            *(u32x4_t*)(a.out + (size_t)at.token * a.ldo_b + (size_t)at.head * 256 + c * 16) = pack8(acc);
         } else {
             const size_t row = (size_t)tr.range * a.T * a.n_q + (size_t)at.token * a.n_q + at.head;
-            float* op = a.po + row * HEAD_DIM + ch0 * 4;
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) *(f32x4_t*)(op + 4 * q4) = (f32x4_t){acc[4 * q4], acc[4 * q4 + 1], acc[4 * q4 + 2], acc[4 * q4 + 3]};
-            if ((lane & 7) == 0) *(f32x2_t*)(a.pml + row * 2) = (f32x2_t){mm, ll};
+            float* op = a.po + row * HEAD_DIM + c * 8;
+            *(f32x4_t*)op = (f32x4_t){acc[0], acc[1], acc[2], acc[3]};
+            *(f32x4_t*)(op + 4) = (f32x4_t){acc[4], acc[5], acc[6], acc[7]};
+            if (c == 0) *(f32x2_t*)(a.pml + row * 2) = (f32x2_t){mm, ll};
         }
     }
 }
@@ -596,6 +571,35 @@ __global__ __launch_bounds__(256, RG == 1 ? 2 : 1) void paged_attn_few_kernel(At
 // Many rows: NW waves of 32 rows each share a double-buffered stream of 64-key tiles.
 constexpr int MANY_TILE = 64;
 constexpr int MANY_BUF = 2 * MANY_TILE * 256;                   // K and V image: 32 KiB
+
+// LDS writes done, then the barrier; global loads on their way to registers stay in flight (__syncthreads would wait for them)
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// MFMA fragments out of the images (v_mfma_f32_32x32x16_bf16).
+//   K (A operand of S^T, 32 keys x 16 features): lane -> key 32 k2 + (lane & 31), chunk 2 ks + (lane >> 5)
+//   V^T (A operand of O^T, 32 features x 16 keys): keys 16 st + 4 h .. + 3 and + 8, features 32 db + (lane & 31)
+struct ImageReader {
+    int k0, v0;
+    __device__ __forceinline__ explicit ImageReader(int lane) {
+        const int c = lane & 31, h = lane >> 5;
+        k0 = c * 256 + ((h ^ swz(c)) << 4);
+        const int i16 = lane & 15, tq = i16 >> 2, tp = i16 & 3;
+        const int ch = 2 * ((lane >> 4) & 1) + (tp >> 1);
+        v0 = (4 * h + tq) * 256 + ((ch ^ swz(4 * h + tq)) << 4) + 8 * (tp & 1);
+    }
+    __device__ __forceinline__ bf16x8_t k(const char* img, int k2, int ks) const {
+        return *(const bf16x8_t*)(img + 32 * k2 * 256 + (k0 ^ (ks << 5)));
+    }
+    __device__ __forceinline__ bf16x8_t v(const char* img, int st, int db) const {
+        const char* p = img + st * 4096;
+        const int at = v0 ^ (db << 6);
+        return join4(read_transposed(p + at), read_transposed(p + 2048 + (at ^ (swz(8) << 4))));
+    }
+};
 
 template <int NW, bool F8, bool G16>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kernel(AttnArgs a) {
@@ -612,8 +616,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
     Limits lm;
     if (!find_unit<R>(a, blockIdx.x / a.n_kv, tr, lm)) return;
     const int last = min(tr.r0 + R, tr.rows) - 1;
-    const int end = limit_of(a, lm, fast_div(a.gdiv, last));
-    const int all = limit_of(a, lm, fast_div(a.gdiv, tr.r0));
+    const int end = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, last)));
+    const int all = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, tr.r0)));
     const int nsp = a.max_ranges > 1 ? max(1, (end + tr.keys - 1) / tr.keys) : 1;
     if (tr.range >= nsp) return;
     const int k_lo = tr.range * tr.keys, k_hi = min(end, k_lo + tr.keys);
@@ -642,15 +646,19 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
     unsigned long long bad = 0;
 
     u32x4_t kr[NP], vr[NP];
-    TileSource<MANY_TILE, NP, NW, F8, G16> src;
-    src.first = wave;
-    auto fetch = [&] {
+    PageSource<MANY_TILE, G16> src;
+    auto fetch = [&](int t) {                                   // pieces i NW + wave of tile t; returns which of its keys exist
+        src.advance(a, table, k_lo, k_hi, t, 1);
+        constexpr int ROW = F8 ? 128 : 256, PROWS = F8 ? 8 : 4, SUB = F8 ? 8 : 16;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const size_t off = src.at(i);
-            kr[i] = *(const u32x4_t*)(kbase + off);
-            vr[i] = *(const u32x4_t*)(vbase + off);
+            const int key = (i * NW + wave) * PROWS;
+            const size_t at = G16 ? src.group(t, key >> 4) : src.key(key + lane / SUB);
+            const unsigned int in = G16 ? (key & 15) * ROW + lane * 16 : (lane % SUB) * 16;
+            kr[i] = *(const u32x4_t*)(kbase + at + in);
+            vr[i] = *(const u32x4_t*)(vbase + at + in);
         }
+        return src.exist(k_lo, k_hi, t);
     };
     const ImageWriter<F8> img(lane);
     const ImageReader rd(lane);
@@ -719,8 +727,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
     if (threadIdx.x < 4) dropped_s[threadIdx.x] = 0;
     __syncthreads();
     if (nt > 0) {
-        auto resolve = [&](int t) { src.resolve(a, k_lo + t * MANY_TILE, k_hi); };
-        auto look_up = [&](int t) { src.look_up(a, table, k_lo + t * MANY_TILE, k_hi); };
         // registers -> image of tile t; partly seen by the WORKGROUP's rows: it must hold finite values and zeros only
         auto publish = [&](int t, unsigned long long ok) {
             char* kimg = lds + (t & 1) * MANY_BUF;
@@ -728,54 +734,53 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
             if (ok != ~0ull || k_lo + (t + 1) * MANY_TILE > all) {
                 bool dropped = false;
 #pragma unroll
-                for (int i = 0; i < NP; ++i) dropped |= img.template put<true>(kimg, vimg, i * NW + wave, kr[i], vr[i], ok);
+                for (int i = 0; i < NP; ++i) {
+                    img.template put<false>(kimg, i * NW + wave, kr[i], ok);
+                    dropped |= img.template put<true>(vimg, i * NW + wave, vr[i], ok);
+                }
                 if (dropped) dropped_s[t & 3] = 1;
             } else {
 #pragma unroll
-                for (int i = 0; i < NP; ++i) img.template put<false>(kimg, vimg, i * NW + wave, kr[i], vr[i], ok);
+                for (int i = 0; i < NP; ++i) {
+                    img.template put<false>(kimg, i * NW + wave, kr[i], ok);
+                    img.template put<false>(vimg, i * NW + wave, vr[i], ok);
+                }
             }
         };
-        look_up(0);
-        resolve(0);
-        fetch();
-        look_up(1);
-        unsigned long long ok = src.ok, ok_next = 0;
+        src.start(a, table, k_lo, k_hi, 0);
+        unsigned long long ok = fetch(0), ok_next = 0;
         publish(0, ok);
-        if (nt > 1) {
-            resolve(1);
-            fetch();
-            ok_next = src.ok;
-            look_up(2);
-        }
+        if (nt > 1) ok_next = fetch(1);
         for (int t = 0; t < nt; ++t) {
             // one barrier a tile: behind it tile t's image is complete and nobody reads tile t - 1's any more
-            __syncthreads();
+            lds_barrier();
             const bool dropped = dropped_s[t & 3] != 0;
             if (threadIdx.x == 0) dropped_s[(t + 2) & 3] = 0;   // last read two barriers ago, next written behind the next one
             unsigned long long ok_after = 0;
             if (t + 1 < nt) {
                 publish(t + 1, ok_next);
                 __builtin_amdgcn_sched_barrier(0);
-                if (t + 2 < nt) {
-                    resolve(t + 2);
-                    fetch();
-                    ok_after = src.ok;
-                    look_up(t + 3);
-                }
+                if (t + 2 < nt) ok_after = fetch(t + 2);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const char* kimg = lds + (t & 1) * MANY_BUF;
             const int key0 = k_lo + t * MANY_TILE;
             if (key0 < w_any) {                                 // else none of this wave's rows sees the tile
                 tile(t, kimg, ok != ~0ull || key0 + MANY_TILE > w_all, ok);
-                if (dropped) bad |= find_nonfinite<F8>(a, table, head_off, key0, MANY_TILE, k_hi, lim, h);
+                if (dropped)
+                    bad |= find_nonfinite<F8>(a, table, head_off, key0, MANY_TILE, k_hi, lim, 64,
+                                              [&](int e) { return 32 * (e >> 4) + (e & 3) + 8 * ((e >> 2) & 3) + 4 * h; });
             }
             ok = ok_next;
             ok_next = ok_after;
         }
     }
 
-    poison(o, bad);
+    if (__any(bad != 0)) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+            if ((bad >> e) & 1) o[e >> 4][e & 15] = __builtin_nanf("");
+    }
     // ---- epilogue (flash_attn.hip): the halves trade groups so that a lane holds 8 consecutive features
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
     const bool live = my_row < tr.rows;
@@ -812,9 +817,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
 // number of ranges).  Up to FEW_RANGES ranges: a wave per row, every range's loads in flight at once; more: a workgroup per row, the
 // ranges shared out over its eight half-waves, which meet in LDS.
 constexpr int FEW_RANGES = 8;
-
-// weight of a part with maximum m in a sum with maximum mm; a part without a maximum holds zeros (or NaN): nothing to scale
-__device__ __forceinline__ float part_weight(float m, float mm) { return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mm); }
 
 template <int R>
 __device__ __forceinline__ int ranges_of(const AttnArgs& a, int token, int head) {
@@ -919,10 +921,10 @@ Plan make_plan(int T, int B, int max_kv, int n_q, int n_kv, int cus) {
     const int g = n_q / n_kv;
     const double rho = (double)T * g / B;                       // rows per sequence and key/value head, on average
     Plan p;
-    p.R = rho <= 32 ? 32 : rho <= 64 ? 64 : rho <= 128 ? 128 : 256;
+    p.R = rho <= 16 ? 16 : rho <= 32 ? 32 : rho <= 64 ? 64 : rho <= 128 ? 128 : 256;
     const long long bound = (long long)T * g / p.R + B;         // tiles per key/value head, at most
     const long long some = ((long long)T * g + p.R - 1) / p.R > B ? ((long long)T * g + p.R - 1) / p.R : B;   // and where no sequence is empty, at least
-    const long long slots = (p.R == 32 || p.R == 128 ? 2 : 1) * (long long)cus;          // workgroups resident at once
+    const long long slots = (p.R <= 32 || p.R == 128 ? 2 : 1) * (long long)cus;          // workgroups resident at once
     // no range under eight steps of a workgroup (the second kernel and a short range's start cost as much), and no more partial outputs
     // than 64 MiB
     const int least = p.R <= 64 ? 1024 : 512;
@@ -999,8 +1001,9 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     // pages of a multiple of 16 keys take the kernels that address 16 keys at a time
     auto pick = [&](auto f8c, auto g16c) -> int {
         constexpr bool F8 = decltype(f8c)::value, G16 = decltype(g16c)::value;
-        if (p.R == 32) return go(paged_attn_few_kernel<1, F8, G16>, 256, 4 * FEW_WAVE_LDS);
-        if (p.R == 64) return go(paged_attn_few_kernel<2, F8, G16>, 256, 4 * FEW_WAVE_LDS);
+        if (p.R == 16) return go(paged_attn_few_kernel<1, 1, F8, G16>, 256, 4 * FEW_WAVE_LDS);
+        if (p.R == 32) return go(paged_attn_few_kernel<2, 1, F8, G16>, 256, 4 * FEW_WAVE_LDS);
+        if (p.R == 64) return go(paged_attn_few_kernel<2, 2, F8, G16>, 512, 8 * FEW_WAVE_LDS);
         if (p.R == 128) return go(paged_attn_many_kernel<4, F8, G16>, 256, 2 * MANY_BUF);
         return go(paged_attn_many_kernel<8, F8, G16>, 512, 2 * MANY_BUF);
     };
@@ -1015,7 +1018,8 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
         if (p.max_ranges <= FEW_RANGES) hipLaunchKernelGGL(paged_attn_join_few_kernel<R>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
         else hipLaunchKernelGGL(paged_attn_join_kernel<R>, dim3((unsigned)rows), dim3(256), 0, st, a);
     };
-    if (p.R == 32) join(std::integral_constant<int, 32>{});
+    if (p.R == 16) join(std::integral_constant<int, 16>{});
+    else if (p.R == 32) join(std::integral_constant<int, 32>{});
     else if (p.R == 64) join(std::integral_constant<int, 64>{});
     else if (p.R == 128) join(std::integral_constant<int, 128>{});
     else join(std::integral_constant<int, 256>{});
