@@ -72,10 +72,55 @@ __device__ __forceinline__ int keys_of(int kv, int range_keys) {
     return ((kv + n - 1) / n + 127) & ~127;
 }
 
+// Uncut calls with a mask: tiles are taken longest first, over all sequences, so that the last ones to start are short (eight causal
+// sequences of 2048 tokens are 1024 tiles of 1 .. 16 lengths on 256 CUs: in sequence order the last CU ends 19 % after the average).
+// Tile k of a sequence sees about min(kv, pos0 + (k + 1) R / g) keys, which grows with k, so how many of its tiles see at least `keys`
+// is a formula and the order needs no sorting: lane j counts the tiles of at least the j-th of 33 thresholds.  For up to 16 sequences: the
+// search walks over all of them, and tiles of one sequence that run at different times no longer find its keys in the L2 (us with / without:
+// 4 x 2048 tokens 94 / 121, 8 x 2048 179 / 203, 16 x 1000 behind 500 196 / 204, but 30 x 600 125 / 106, 32 x 384 78 / 65).
+constexpr int LONGEST_FIRST = 16, LEVELS = 32;
+
+struct Cost {
+    int tiles, kv, pos0;                       // of one sequence
+    template <int R>
+    __device__ __forceinline__ int at_least(const AttnArgs& a, int keys) const {       // tiles that see `keys` or more
+        if (kv < keys) return 0;
+        const long long need = max((long long)keys - pos0, 0ll) * a.g;
+        return max(tiles - max((int)min((need + R - 1) / R, 0x7fffffffll) - 1, 0), 0);
+    }
+};
+
+// -> the sequence, k: its tile; b = -1: none
+template <int R>
+__device__ __forceinline__ Seq longest_first(const AttnArgs& a, const SeqLane& l, int item, int& k) {
+    const int lane = threadIdx.x & 63;
+    const Cost mine = {tiles_of<R>(l, a.g), kv_of(a, l.x), max(l.y, 0)};
+    auto of = [&](int b) {
+        return Cost{__builtin_amdgcn_readlane(mine.tiles, b), __builtin_amdgcn_readlane(mine.kv, b), __builtin_amdgcn_readlane(mine.pos0, b)};
+    };
+    int hi = 0;
+    for (int b = 0; b < a.B; ++b) hi = max(hi, of(b).kv);
+    const int step = hi / LEVELS + 1;
+    auto threshold = [&](int j) { return max(hi + 1 - j * step, 0); };      // none .. all
+    const int keys = threshold(min(lane, LEVELS));
+    int total = 0;
+    for (int b = 0; b < a.B; ++b) total += of(b).template at_least<R>(a, keys);
+    const unsigned long long fewer = __ballot(total <= item);               // a run of ones from lane 0
+    const int j = __popcll(fewer) - 1;
+    k = 0;
+    if (j >= LEVELS) return {-1, 0, 0, 0, 0};
+    const int before = lane < a.B ? mine.at_least<R>(a, threshold(j)) : 0;
+    const int here = lane < a.B ? mine.at_least<R>(a, threshold(j + 1)) - before : 0;
+    const int sum = wave_running_sum(here), left = item - __builtin_amdgcn_readlane(total, j);
+    const int b = __ffsll((long long)__ballot(sum > left)) - 1;
+    k = __builtin_amdgcn_readlane(mine.tiles - 1 - before, b) - (left - __builtin_amdgcn_readlane(sum - here, b));
+    return l.from(b, b);
+}
+
 // Work unit -> tile and range.  The longest a range may be follows from the whole work, sum over the sequences of tiles * keys, so that
 // the units come out about equal and about as many as the chip takes at once (or in a few rounds): every wave adds the lengths up for
 // itself, in the same order.
-template <int R>
+template <int R, bool LONGEST>
 __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, TileRows& t, Limits& lm) {
     const SeqArrays arr = {a.seq_start, a.kv_len, a.pos0, a.B, a.T};
     SeqBlock blk;
@@ -97,17 +142,25 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, TileRows&
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.range_keys = range_keys;
     }
     int k;
-    const Seq q = seq_of_item(arr, blk, unit, k, [&](const SeqLane& l) {
-        const int kv = kv_of(a, l.x);
-        return tiles_of<R>(l, a.g) * (a.max_ranges > 1 ? max(1, (kv + range_keys - 1) / range_keys) : 1);
-    });
+    Seq q;
+    if (LONGEST && a.max_ranges == 1 && a.mask_block && a.B <= LONGEST_FIRST) {
+        q = longest_first<R>(a, blk.l[0], unit, k);
+    } else {
+        q = seq_of_item(arr, blk, unit, k, [&](const SeqLane& l) {
+            const int kv = kv_of(a, l.x);
+            return tiles_of<R>(l, a.g) * (a.max_ranges > 1 ? max(1, (kv + range_keys - 1) / range_keys) : 1);
+        });
+        // later tiles of a sequence see more keys under a mask: they go first
+        const int ranges = max(1, (kv_of(a, q.x) + range_keys - 1) / range_keys), rows = q.n * a.g, tiles = rows / R + (rows % R != 0);
+        k = (tiles - 1 - k / ranges) * ranges + k % ranges;
+    }
     if (__builtin_amdgcn_readfirstlane(q.b) < 0) return false;
     lm = limits_of(a, q);
-    const int rows = q.n * a.g, tiles = rows / R + (rows % R != 0), ranges = max(1, (lm.kv + range_keys - 1) / range_keys);
-    // Later tiles see more keys under a mask: they go first.  All of this is the same in every lane, which the compiler does not find out
-    // by itself (loops, ballots): told so, it keeps what follows from it - bounds, page bases, branches - in scalar registers.
+    const int rows = q.n * a.g, ranges = max(1, (lm.kv + range_keys - 1) / range_keys);
+    // All of this is the same in every lane, which the compiler does not find out by itself (loops, ballots): told so, it keeps what
+    // follows from it - bounds, page bases, branches - in scalar registers.
     auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    t = {u(q.b), u(q.s0), u(q.n), u((tiles - 1 - k / ranges) * R), u(rows), u(k % ranges), u(keys_of(lm.kv, range_keys))};
+    t = {u(q.b), u(q.s0), u(q.n), u(k / ranges * R), u(rows), u(k % ranges), u(keys_of(lm.kv, range_keys))};
     lm = {u(lm.kv), u(lm.pos0)};
     return true;
 }
@@ -338,7 +391,7 @@ __global__ __launch_bounds__(256 * RW, RG == 1 && F8 ? 3 : 2) void paged_attn_fe
     const int kvh = blockIdx.x % a.n_kv;
     TileRows tr;
     Limits lm;
-    if (!find_unit<R>(a, blockIdx.x / a.n_kv, tr, lm)) return;
+    if (!find_unit<R, false>(a, blockIdx.x / a.n_kv, tr, lm)) return;
     const int last = min(tr.r0 + R, tr.rows) - 1;               // last live row of the tile
     const int end = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, last)));    // keys that any row of the tile sees
     const int all = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, tr.r0)));   // keys that every row of it sees
@@ -614,7 +667,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
     const int kvh = blockIdx.x % a.n_kv;
     TileRows tr;
     Limits lm;
-    if (!find_unit<R>(a, blockIdx.x / a.n_kv, tr, lm)) return;
+    if (!find_unit<R, true>(a, blockIdx.x / a.n_kv, tr, lm)) return;
     const int last = min(tr.r0 + R, tr.rows) - 1;
     const int end = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, last)));
     const int all = __builtin_amdgcn_readfirstlane(limit_of(a, lm, fast_div(a.gdiv, tr.r0)));
@@ -962,7 +1015,8 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     const char* who = "coda_paged_attn";
     if (B <= 0 || T <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv) return coda_refuse(who, CODA_ERR_SHAPE, "a size is not positive, or n_q % n_kv");
     if ((long long)T * n_q > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "T * n_q exceeds 2^31 - 1");
-    if (max_kv < 0 || (long long)max_kv > (long long)max_pages * page_size) return coda_refuse(who, CODA_ERR_SHAPE, "max_kv is not within max_pages * page_size");
+    if (max_kv < 0 || (long long)max_kv > (long long)max_pages * page_size || max_kv > 1 << 30)
+        return coda_refuse(who, CODA_ERR_SHAPE, "max_kv is not within max_pages * page_size and 2^30");
     if (ld_q < (long long)n_q * HEAD_DIM || ld_out < (long long)n_q * HEAD_DIM) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");
     if (!q || !out || !seq_start || !pos0 || !kv_len) return coda_refuse(who, CODA_ERR_ARG, "null pointer");
     if (!(scale > 0.f) || scale > 1e30f) return coda_refuse(who, CODA_ERR_ARG, "scale must be positive and finite");

@@ -273,7 +273,7 @@ int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out, long long 
  * (the denoiser's attention).  mask_block m > 0: token i sees the keys before the end of its block of m positions,
  * j < ((pos0[b] + i) / m + 1) * m (1: causal).  A token that sees no key gets zeros.  Keys a token does not see
  * have no influence on it, whatever their slots hold; an infinity or NaN that it does see makes its output non-finite.
- * max_kv: host-side bound of kv_len, at most max_pages * page_size (keys from max_kv on are not seen): it sizes the launch.
+ * max_kv: host-side bound of kv_len, at most max_pages * page_size and 2^30 (keys from max_kv on are not seen): it sizes the launch.
  * Scores, maxima, sums and outputs are fp32; weights enter the second product as bf16 (a bf16 pair where there are at most 64
  * rows per sequence and key/value head).  scale > 0.
  * workspace: coda_paged_attn_workspace_bytes(T, B, max_kv, n_q, n_kv) bytes (may be 0), 16-byte aligned, contents irrelevant before

@@ -452,3 +452,19 @@ def test_append_e4m3_saturates_and_keeps_nan():
     assert got[0, 0] == 448 and got[0, 1] == -448 and torch.isnan(got[0, 2]) and got[1, 0] == 448 and got[1, 1] == -448
     got = b.pages(k.view(torch.uint8))[page, 0].contiguous().view(F8).float()
     assert got[2, 0] == 448 and got[2, 1] == -240 and (got[2, 2:] == 0).all()
+
+
+@pytest.mark.parametrize("mask", [1, 64])
+@pytest.mark.parametrize("B", [2, 9, 16, 17])
+def test_attention_tile_order(B, mask):
+    """Long prompts of very different lengths and pasts, masked: every tile of every sequence is done, whatever order they are taken
+    in (up to 16 sequences longest first, more in sequence order)."""
+    lens = [(i * 97) % 260 for i in range(B)]
+    lens[0], lens[1] = 300, 131
+    past = [(i * 211) % 500 for i in range(B)]
+    b = Batch(lens, past, 64, 2, 1, seed=71)
+    b.pos0[1] = -40                                          # the first 40 tokens see nothing
+    check(attn(b, mask), b, mask=mask)
+    b.pos0[0] = 10 ** 6                                      # far behind every key: all rows see all of them
+    b.kv_len[2 % B] = 0
+    check(attn(b, mask), b, mask=mask)
