@@ -2,7 +2,7 @@
 //
 //     C[t] = R[t] + s[a] (X[t] A[a]^T) B[a]^T,     a = the adapter of t's sequence;  no adapter: C[t] = R[t]
 //
-// Two launches.  `down` computes U = X A^T for tiles of one sequence's tokens, K cut over the waves of a workgroup and, where there
+// Two launches (one for small batches, lora_one_kernel).  `down` computes U = X A^T for tiles of one sequence's tokens, K cut over the waves of a workgroup and, where there
 // are few tiles, over workgroups (fp32 slabs in the workspace, summed in a fixed order by their readers).  `up` sums the slabs, scales, and
 // adds U B^T to R with R as the start value of the accumulators, so that the result is rounded once.
 //
@@ -248,7 +248,108 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
     }
 }
 
+// Both products of 16 tokens in one launch, for batches that wait for latency and not for bytes (single tokens of some requests): a
+// workgroup of 16 waves takes 1024 features of a tile and computes the tile's U for itself, K cut over the waves, fragments straight from
+// memory with everything in flight at once: weights and R of the second product while the first one runs.
+template <int RT>
+__global__ __launch_bounds__(1024) void lora_one_kernel(LoraArgs a) {
+    __shared__ f32x4_t part[16][RT][64];
+    __shared__ __attribute__((aligned(16))) __bf16 us[2][16][40];        // rows of 32 ranks, padded
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const int nsl = (a.N + 1023) / 1024, n0 = (int)(blockIdx.x % nsl) * 1024;
+    const Tile t = find_tile<16>(a, blockIdx.x / nsl);
+    if (t.n == 0) return;
+    const int f0 = n0 + 64 * wave;
+    const size_t row = t.row0 + min(col, t.n - 1);
+    // R, and the weights of the second product: row m of block j is feature 32 (j >> 1) + 8 (m >> 2) + 4 (j & 1) + (m & 3), so that a
+    // lane's accumulators of two blocks are 8 consecutive features of its token
+    u32x4_t rr[2];
+    bf16x8_t w[4];
+    const char* bp = a.b + (size_t)max(t.adapter, 0) * a.N * a.rank * 2;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) rr[q] = *(const u32x4_t*)(a.r + row * a.ldr_b + (size_t)min(f0 + 32 * q + 8 * quad, a.N - 8) * 2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int f = min(f0 + 32 * (j >> 1) + 8 * (col >> 2) + 4 * (j & 1) + (col & 3), a.N - 1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[j][e] = (__bf16)0.f;
+        if (8 * quad < a.rank) w[j] = *(const bf16x8_t*)(bp + ((size_t)f * a.rank + 8 * quad) * 2);
+    }
+    f32x4_t acc[4];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        float x[8];
+        unpack8(rr[q], x);
+        acc[2 * q] = (f32x4_t){x[0], x[1], x[2], x[3]};
+        acc[2 * q + 1] = (f32x4_t){x[4], x[5], x[6], x[7]};
+    }
+    if (t.adapter >= 0) {
+        const char* xp = a.x + row * a.ldx_b + quad * 16;
+        f32x4_t u[RT];
+        const char* ap[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            u[r] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            ap[r] = a.a + ((size_t)t.adapter * a.rank + min(16 * r + col, a.rank - 1)) * a.K * 2 + quad * 16;
+        }
+        for (int k = 64 * wave; k < a.K; k += 2048) {                    // two 128-byte lines of every row per wave and step
+            bf16x8_t xf[4], af[4][RT];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const size_t at = (size_t)min(k + 1024 * (s >> 1), a.K - 64) * 2 + (s & 1) * 64;
+                xf[s] = *(const bf16x8_t*)(xp + at);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) af[s][r] = *(const bf16x8_t*)(ap[r] + at);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (k + 1024 * (s >> 1) < a.K) {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) u[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[s][r], xf[s], u[r], 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) part[wave][r][lane] = u[r];
+        __syncthreads();
+        if (wave < 2) {                                                  // ranks 16 wave + 4 quad .. + 3 of token col
+            f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+            if (wave < RT && 16 * wave + 4 * quad < a.rank) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v += part[i][wave < RT ? wave : 0][lane];
+            }
+            const float s = a.scale ? a.scale[t.adapter] : 1.0f;
+            bf16x4_t h4, l4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = s * v[j];
+                h4[j] = (__bf16)x;
+                l4[j] = (__bf16)(x - (float)h4[j]);
+            }
+            *(bf16x4_t*)&us[0][col][16 * wave + 4 * quad] = h4;
+            *(bf16x4_t*)&us[1][col][16 * wave + 4 * quad] = l4;
+        }
+        __syncthreads();
+        const bf16x8_t hi = *(const bf16x8_t*)&us[0][col][8 * quad], lo = *(const bf16x8_t*)&us[1][col][8 * quad];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j], lo, acc[j], 0, 0, 0);
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j], hi, acc[j], 0, 0, 0);
+        }
+    } else if (a.r == a.c && a.ldr_b == a.ldc_b) {
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int f = f0 + 32 * q + 8 * quad;
+        const u32x4_t v = {pack_bf16x2(acc[2 * q][0], acc[2 * q][1]), pack_bf16x2(acc[2 * q][2], acc[2 * q][3]),
+                           pack_bf16x2(acc[2 * q + 1][0], acc[2 * q + 1][1]), pack_bf16x2(acc[2 * q + 1][2], acc[2 * q + 1][3])};
+        if (col < t.n && f < a.N) *(u32x4_t*)(a.c + row * a.ldc_b + (size_t)f * 2) = v;
+    }
+}
+
 struct Plan {
+    bool one;                                   // one launch
     int mt, ksplit, kchunk, nslice;             // mt: 16-token blocks per tile
     long long nslots;
 };
@@ -260,6 +361,9 @@ Plan make_plan(int T, int B, int N, int K, int rank, int cus) {
     p.mt = (double)T / B <= 16 ? 1 : 2;
     p.nslots = (long long)T / (16 * p.mt) + B;
     const long long tiles = ((long long)T + 16 * p.mt - 1) / (16 * p.mt) > B ? ((long long)T + 16 * p.mt - 1) / (16 * p.mt) : B;
+    // One launch where a CU gets at most one workgroup of it and the A that each of them reads is small: us a call one / two launches, rank 16,
+    // 2048 -> 4096: 8.3 / 11.0 with 64 single tokens (256 workgroups), 13.2 / 11.1 with 128; rank 16, 6144 -> 2048 (A of 98 k values): equal
+    p.one = p.mt == 1 && rank <= 32 && (long long)rank * K <= 65536 && tiles * ((N + 1023) / 1024) <= cus;
     // features of a workgroup: two steps where that leaves a workgroup per CU (U is put together once for both: 135 us against 143 on the
     // same prompts, and four steps 138), else one
     p.nslice = tiles * ((N + 511) / 512) >= cus ? 512 : 256;
@@ -277,7 +381,7 @@ Plan make_plan(int T, int B, int N, int K, int rank, int cus) {
     return p;
 }
 
-long long plan_bytes(const Plan& p, int T, int rank) { return p.nslots * (long long)sizeof(Tile) + (long long)p.ksplit * T * rank * 4; }
+long long plan_bytes(const Plan& p, int T, int rank) { return p.one ? 0 : p.nslots * (long long)sizeof(Tile) + (long long)p.ksplit * T * rank * 4; }
 
 }  // namespace
 
@@ -298,7 +402,7 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
     if (((uintptr_t)X | (uintptr_t)A | (uintptr_t)Bw | (uintptr_t)R | (uintptr_t)C) & 15 || (ldx * 2) % 16 || (ldr * 2) % 16 || (ldc * 2) % 16)
         return coda_refuse(who, CODA_ERR_ALIGN, "rows start on 16 bytes");
     const Plan p = make_plan(T, B, N, K, rank, coda_device_cus());
-    if (!workspace || workspace_bytes < plan_bytes(p, T, rank))
+    if (!p.one && (!workspace || workspace_bytes < plan_bytes(p, T, rank)))
         return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_lora_workspace_bytes");
     if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
     const long long downs = p.nslots * p.ksplit, ups = p.nslots * ((N + p.nslice - 1) / p.nslice);
@@ -315,6 +419,13 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
     a.u = (float*)(a.tiles + p.nslots);
     hipStream_t st = (hipStream_t)stream;
     const dim3 gd((unsigned)downs), gu((unsigned)ups), block(256);
+    if (p.one) {
+        const dim3 g1((unsigned)(p.nslots * ((N + 1023) / 1024)));
+        if (rank <= 16) hipLaunchKernelGGL(lora_one_kernel<1>, g1, dim3(1024), 0, st, a);
+        else hipLaunchKernelGGL(lora_one_kernel<2>, g1, dim3(1024), 0, st, a);
+        CODA_CHECK_LAUNCH("lora");
+        return CODA_OK;
+    }
     auto down = [&](auto kernel, int lds) -> int {
         if (coda_ensure_dyn_lds((const void*)kernel, lds) != CODA_OK) return CODA_ERR_LAUNCH;
         hipLaunchKernelGGL(kernel, gd, block, lds, st, a);

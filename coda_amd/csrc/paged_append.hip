@@ -71,6 +71,20 @@ __device__ __forceinline__ u32x2_t pack_e4m3(const float (&f)[8]) {
     return o;
 }
 
+// lane -> the lane `N` further on, round its group of 16: a register move, where __shfl_xor goes through LDS
+template <int N>
+__device__ __forceinline__ float rotate16(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x120 + N, 0xf, 0xf, false));
+}
+
+// sum over the 16 lanes of a row, in the pairs (and with the bits) of a butterfly of 8, 4, 2, 1
+__device__ __forceinline__ float row_sum(float v) {
+    v += rotate16<8>(v);
+    v += rotate16<4>(v);
+    v += rotate16<2>(v);
+    return v + rotate16<1>(v);
+}
+
 // F8: e4m3 cache.  STEPWISE: bf16 after every operation, the rounding points (and bits) of coda_qknorm_rope; otherwise
 // everything stays in fp32 and is rounded once, to the type it is stored in.
 template <bool F8, bool STEPWISE>
@@ -80,6 +94,16 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     const long long tl = wave / a.parts;
     if (tl >= a.T) return;
     const int t = __builtin_amdgcn_readfirstlane((int)tl), part = __builtin_amdgcn_readfirstlane((int)(wave - tl * a.parts));
+    const char* row = a.qkv + (size_t)t * a.ld_b + sub * 16;
+    const int n_heads = a.n_q + 2 * a.n_kv, step = 4 * a.parts;
+    // four rows of loads in flight per lane, the first before anything is known about the token; a row beyond the last head re-reads the
+    // last one and stores nothing
+    u32x4_t raw[4];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) raw[u] = *(const u32x4_t*)(row + (size_t)min(h0 + u * step, n_heads - 1) * 256);
+    };
+    load(part * 4 + grp);
     const Seq q = seq_of_token({a.seq_start, a.pos0, nullptr, a.B, a.T}, t);
     if (q.b < 0) return;                                        // a row of no sequence: left alone
     const int b = q.b;
@@ -94,10 +118,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     float c[8], s[8];
     unpack8(a.cos[(size_t)pos * 16 + sub], c);
     unpack8(a.sin[(size_t)pos * 16 + sub], s);
-    const float sign = sub < 8 ? -1.0f : 1.0f;                  // the first half takes -x2, the second half x1
-    const char* row = a.qkv + (size_t)t * a.ld_b + sub * 16;
+    if (sub < 8) {                                              // the first half takes -x2, the second half x1
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = -s[j];
+    }
     char* qrow = a.q_out + (size_t)t * a.ldq_b + sub * 16;
-    const int n_heads = a.n_q + 2 * a.n_kv;
 
     auto put = [&](char* cache, int h, const float (&y)[8], float inv) {
         char* dst = cache + at + (size_t)h * a.pg.head_stride_b;
@@ -116,16 +141,20 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     auto one = [&](int h, const u32x4_t raw) {
         float f[8];
         unpack8(raw, f);
-        // the four rows of a wave can be of different kinds, and the shuffles below need every lane: v rows run along
+        if (h - grp >= a.n_q + a.n_kv) {                        // four v rows: wave-uniform
+            if (h < n_heads && store) put(a.v, h - a.n_q - a.n_kv, f, a.v_inv);
+            return;
+        }
+        // the four rows of a wave can be of different kinds, and the exchanges below need every lane: v rows run along
         const bool is_q = h < a.n_q, is_v = h >= a.n_q + a.n_kv;
         float n[8], other[8], y[8];
         if (a.qw) {
             float ss = 0.f, w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            const float inv = 1.0f / sqrtf(ss * (1.0f / 128.0f) + a.eps);
+            const float ms = row_sum(ss) * (1.0f / 128.0f) + a.eps;
+            // the reciprocal root instruction is off by one last place, far below the stored type's; the stepwise form keeps the exact one
+            const float inv = STEPWISE ? 1.0f / sqrtf(ms) : __builtin_amdgcn_rsqf(ms);
             unpack8((is_q ? a.qw : a.kw)[sub], w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) n[j] = STEPWISE ? round_bf16(w[j] * round_bf16(f[j] * inv)) : w[j] * (f[j] * inv);
@@ -134,11 +163,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
             for (int j = 0; j < 8; ++j) n[j] = f[j];
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) other[j] = __shfl_xor(n[j], 8, 64);
+        for (int j = 0; j < 8; ++j) other[j] = rotate16<8>(n[j]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (STEPWISE) y[j] = round_bf16(round_bf16(n[j] * c[j]) + round_bf16(sign * other[j] * s[j]));
-            else y[j] = n[j] * c[j] + sign * other[j] * s[j];
+            if (STEPWISE) y[j] = round_bf16(round_bf16(n[j] * c[j]) + round_bf16(other[j] * s[j]));
+            else y[j] = n[j] * c[j] + other[j] * s[j];
         }
         if (h >= n_heads) return;
         if (is_q) {
@@ -151,12 +180,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
             else put(a.k, h - a.n_q, y, a.k_inv);
         }
     };
-    // four rows of loads in flight per lane; a row beyond the last head re-reads the last one and stores nothing
-    const int step = 4 * a.parts;
     for (int h0 = part * 4 + grp; h0 - grp < n_heads; h0 += 4 * step) {
-        u32x4_t raw[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) raw[u] = *(const u32x4_t*)(row + (size_t)min(h0 + u * step, n_heads - 1) * 256);
+        if (h0 - grp != part * 4) load(h0);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (h0 - grp + u * step < n_heads) one(h0 + u * step, raw[u]);        // wave-uniform

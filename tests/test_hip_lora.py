@@ -42,7 +42,7 @@ class Case:
             out = torch.full_like(d["r"], float("nan"))
         size = _lib.load().coda_lora_workspace_bytes(self.T, self.B, self.N, self.K, self.rank)
         if ws is None:
-            ws = torch.full((size,), 255, dtype=torch.uint8, device=DEV)       # NaN patterns
+            ws = torch.full((max(size, 16),), 255, dtype=torch.uint8, device=DEV)       # NaN patterns
         _lib.call("coda_lora_bf16", d["x"].data_ptr(), d["x"].stride(0), d["a"].data_ptr(), d["b"].data_ptr(),
                   None if d["scale"] is None else d["scale"].data_ptr(), d["seq_start"].data_ptr(), d["adapter"].data_ptr(), self.B,
                   self.T, self.n, self.rank, d["r"].data_ptr(), d["r"].stride(0), out.data_ptr(), out.stride(0), self.N, self.K,
@@ -136,3 +136,16 @@ def test_lora_same_bits_streams_and_graph():
         got = out.clone()
         assert torch.equal(got[:c.live], c.call()[:c.live])
         c.check(got)
+
+
+@pytest.mark.parametrize("rank", [8, 16, 24, 32])
+@pytest.mark.parametrize("K,N", [(64, 1032), (1984, 264), (2048, 4096), (8192, 72)])
+def test_lora_one_launch(K, N, rank):
+    """Short sequences, small adapters: the single launch (no workspace), against the same bound; 33 sequences so that some tiles are
+    alone on their CU and some are not."""
+    lens = [(i * 5) % 4 for i in range(33)]
+    lens[7] = 21                                             # two tiles
+    c = Case(lens, [(i * 3) % 5 - 1 for i in range(33)], K, N, rank, seed=rank, pad=8)
+    assert (_lib.load().coda_lora_workspace_bytes(c.T, c.B, N, K, rank) == 0) == (rank * K <= 65536)
+    c.check(c.call())
+    c.check(c.call(in_place=True))

@@ -89,7 +89,7 @@ def test_attn_workspace_sizes():
         assert n == 0 or (n - 256) % (T * 16 * 130 * 4) == 0 and n - 256 <= min(kv // 512 * T * 16 * 130 * 4, 64 << 20)
 
 
-LORA = dict(X=P, ldx=256, A=P, Bw=P, scale=None, seq_start=P, adapter=P, B=2, T=4, n_adapters=3, rank=16, R=P, ldr=512, C=P, ldc=512, N=512,
+LORA = dict(X=P, ldx=256, A=P, Bw=P, scale=None, seq_start=P, adapter=P, B=2, T=4, n_adapters=3, rank=64, R=P, ldr=512, C=P, ldc=512, N=512,
             K=256, workspace=P, workspace_bytes=1 << 30, stream=None)
 
 
@@ -110,7 +110,8 @@ def test_lora_refuses(change, code, words):
 def test_lora_workspace_sizes():
     size = _lib.load().coda_lora_workspace_bytes
     assert size(0, 1, 512, 256, 16) == 0 and size(4, 2, 512, 256, 0) == 0
-    for T, B, K, rank in ((1, 1, 2048, 16), (32, 32, 2048, 16), (1024, 32, 6144, 64), (16384, 32, 2048, 128)):
+    assert size(32, 32, 4096, 2048, 16) == 0                                  # single tokens, small adapters: one launch, no slabs
+    for T, B, K, rank in ((1, 1, 6144, 16), (32, 32, 2048, 64), (1024, 32, 6144, 64), (16384, 32, 2048, 128)):
         # 16 bytes a tile (at most T / 16 + B of them), and U in at most K / 256 slabs of fp32
         n = size(T, B, 2048, K, rank)
         assert T * rank * 4 < n <= (T // 16 + B) * 16 + K // 256 * T * rank * 4
