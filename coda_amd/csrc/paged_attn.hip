@@ -69,7 +69,7 @@ __device__ __forceinline__ Limits limits_of(const AttnArgs& a, const Seq& q) { r
 // Length of the ranges of a sequence with kv keys: ceil(kv / range_keys) equal ones, in whole 128 keys
 __device__ __forceinline__ int keys_of(int kv, int range_keys) {
     const int n = max(1, (kv + range_keys - 1) / range_keys);
-    return ((kv + n - 1) / n + 127) & ~127;
+    return max(((kv + n - 1) / n + 127) & ~127, 128);           // also for no keys: it is divided by
 }
 
 // Uncut calls with a mask: tiles are taken longest first, over all sequences, so that the last ones to start are short (eight causal
@@ -1019,19 +1019,21 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
         return coda_refuse(who, CODA_ERR_SHAPE, "max_kv is not within max_pages * page_size and 2^30");
     if (ld_q < (long long)n_q * HEAD_DIM || ld_out < (long long)n_q * HEAD_DIM) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");
     if (!q || !out || !seq_start || !pos0 || !kv_len) return coda_refuse(who, CODA_ERR_ARG, "null pointer");
-    if (!(scale > 0.f) || scale > 1e30f) return coda_refuse(who, CODA_ERR_ARG, "scale must be positive and finite");
+    if (!(scale > 0.f)) return coda_refuse(who, CODA_ERR_ARG, "scale must be positive");
     if (mask_block < 0) return coda_refuse(who, CODA_ERR_ARG, "mask_block is negative");
     if (((uintptr_t)q | (uintptr_t)out) & 15 || (ld_q * 2) % 16 || (ld_out * 2) % 16) return coda_refuse(who, CODA_ERR_ALIGN, "rows start on 16 bytes");
     AttnArgs a;
     const int rc = coda_check_pages(who, k_cache, v_cache, page_table, ld_table, max_pages, page_stride, num_pages, page_size, cache_type,
                                     k_scale, v_scale, n_kv, &a.pg);
     if (rc != CODA_OK) return rc;
+    const bool f8 = cache_type == CODA_CACHE_E4M3;
+    a.scale_log2e = scale * (f8 ? k_scale : 1.0f) * 1.4426950408889634f;
+    if (!(a.scale_log2e >= 1e-30f && a.scale_log2e <= 1e30f)) return coda_refuse(who, CODA_ERR_ARG, "scale times k_scale is not within [1e-30, 1e30]");
     const Plan p = make_plan(T, B, max_kv, n_q, n_kv, coda_device_cus());
     const long long need = plan_bytes(p, T, n_q);
     if (need > 0 && (!workspace || workspace_bytes < need)) return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_paged_attn_workspace_bytes");
     if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
     if (p.wgs > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
-    const bool f8 = cache_type == CODA_CACHE_E4M3;
     a.q = (const char*)q; a.ldq_b = ld_q * 2;
     a.out = (char*)out; a.ldo_b = ld_out * 2;
     a.seq_start = seq_start; a.pos0 = pos0; a.kv_len = kv_len;
@@ -1039,7 +1041,6 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     a.k = (const char*)k_cache; a.v = (const char*)v_cache;
     a.n_q = n_q; a.n_kv = n_kv; a.g = n_q / n_kv; a.gdiv = make_fast_div((unsigned)a.g);
     a.mask_block = mask_block;
-    a.scale_log2e = scale * (f8 ? k_scale : 1.0f) * 1.4426950408889634f;
     a.v_scale = f8 ? v_scale : 1.0f;
     a.max_ranges = p.max_ranges; a.min_keys = p.min_keys; a.per_range = p.per_range;
     a.range_keys = p.max_ranges > 1 ? (int*)workspace : nullptr;

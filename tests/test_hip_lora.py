@@ -94,9 +94,11 @@ def test_lora_long_k_and_many_sequences():
     c = Case([1, 2], [1, 0], 6144, 136, 64)
     assert _lib.load().coda_lora_workspace_bytes(c.T, c.B, c.N, c.K, c.rank) > c.T * c.rank * 4
     c.check(c.call())
-    lens = [(i * 5) % 4 for i in range(200)]
-    c = Case(lens, [(i * 3) % 5 - 1 for i in range(200)], 128, 72, 16, n=3)
-    c.check(c.call())
+    for B in (200, 600):
+        lens = [(i * 5) % 4 for i in range(B)]
+        for rank in (16, 40):                               # one launch, two launches
+            c = Case(lens, [(i * 3) % 5 - 1 for i in range(B)], 128, 72, rank, n=3)
+            c.check(c.call())
 
 
 def test_lora_nothing_leaks_between_rows():
@@ -149,3 +151,15 @@ def test_lora_one_launch(K, N, rank):
     assert (_lib.load().coda_lora_workspace_bytes(c.T, c.B, N, K, rank) == 0) == (rank * K <= 65536)
     c.check(c.call())
     c.check(c.call(in_place=True))
+
+
+@pytest.mark.parametrize("rank", [16, 64])
+@pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-7, 20, 200, 30], [300, 300, 300, 300]])
+def test_lora_starts_that_make_no_sense(starts, rank):
+    """Starts that decrease or leave [0, T]: rows come out wrong or not at all, and nothing else is touched."""
+    c = Case([30, 30, 30], [0, 1, 2], 128, 72, rank)
+    c.seq_start = torch.tensor(starts, dtype=torch.int32)
+    guard = torch.full((c.T + 64, 72), 7.0, device=DEV, dtype=BF)
+    c.call(out=guard[32:32 + c.T])
+    torch.cuda.synchronize()
+    assert (guard[:32] == 7).all() and (guard[32 + c.T:] == 7).all()

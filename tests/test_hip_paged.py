@@ -172,11 +172,50 @@ def test_attention_ranges_of_keys(lens, past, cache):
         check(attn(b, mask), b, mask=mask)
 
 
-def test_attention_many_sequences():
-    """More sequences than one step of the search covers, most of them without a row."""
-    lens = [(i * 7) % 3 for i in range(150)]
-    b = Batch(lens, [(i * 13) % 40 for i in range(150)], 8, 2, 1, seed=8)
-    check(attn(b, 1), b, mask=1)
+@pytest.mark.parametrize("B,past", [(150, 40), (300, 40), (300, 3000)])
+def test_attention_many_sequences(B, past):
+    """More sequences than one step of the search covers, many of them without a row; the last case cuts the keys into ranges."""
+    lens = [(i * 7) % 3 for i in range(B)]
+    b = Batch(lens, [(i * 1301) % past for i in range(B)], 8, 2, 1, seed=8)
+    for mask in (0, 1):
+        check(attn(b, mask), b, mask=mask)
+
+
+@pytest.mark.parametrize("lens", [[1, 1, 1], [40, 3, 20], [70, 9, 9]])
+def test_attention_no_keys_beside_many(lens):
+    """Ranges of keys, and sequences of the same call with none, one or no page."""
+    b = Batch(lens, [4000, 10, 900], 16, 4, 2, seed=13)
+    b.kv_len[1] = 0
+    b.table[2] = -1
+    for mask in (0, 1):
+        out = attn(b, mask)
+        check(out, b, mask=mask)
+        assert (out[b.starts[1]:b.starts[3]] == 0).all()
+    b.kv_len[0] = 1
+    check(attn(b, 0, max_kv=max(b.total)), b, mask=0)
+
+
+def test_attention_rows_before_the_first_sequence():
+    b = Batch([4, 0, 70], [30, 3, 10], 16, 4, 2, seed=9, spare_rows=5)
+    want = attn(b, 1).clone()
+    b.seq_start += 3
+    b.q = torch.cat((b.q[-3:], b.q[:-3]))
+    out = attn(b, 1)
+    assert torch.isnan(out[:3]).all() and torch.equal(out[3:77], want[:74]) and torch.isnan(out[77:]).all()
+
+
+@pytest.mark.parametrize("starts", [[0, 90, 40, 60], [50, 10, 10, 90], [-7, 20, 200, 30], [300, 300, 300, 300], [-1, -1, -1, -1]])
+def test_attention_starts_that_make_no_sense(starts):
+    """Starts that decrease or leave [0, T]: rows come out wrong or not at all, and nothing else is touched."""
+    b = Batch([30, 30, 30], [20, 70, 40], 16, 4, 2, seed=10)
+    b.seq_start = torch.tensor(starts, dtype=torch.int32)
+    guard = torch.full((b.T + 64, b.n_q * D), 7.0, device=DEV, dtype=BF)
+    attn(b, 1, out=guard[32:32 + b.T])
+    assert (guard[:32] == 7).all() and (guard[32 + b.T:] == 7).all()
+    qkv, qw, kw = inputs(b)
+    cos, sin = rope(300)
+    _, k, v = append(b, qkv, qw, kw, cos, sin)               # positions that follow from such starts may have no page: skipped
+    assert torch.isfinite(k.float()).all() and torch.isfinite(v.float()).all()
 
 
 @pytest.mark.parametrize("page", [16, 10])
@@ -205,13 +244,10 @@ def test_attention_lengths_and_bad_pages(lens, page):
     assert (out[:b.starts[-1]] == 0).all()
 
 
-@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("cache,bad", [("bf16", float("inf")), ("bf16", float("-inf")), ("bf16", float("nan")), ("e4m3", float("nan"))])
 @pytest.mark.parametrize("lens,past", [([3], [40]), ([20, 9], [64, 10]), ([32, 30], [40, 41]), ([60, 2], [13, 90]), ([140], [77])])
-@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
 def test_attention_nonfinite_where_nobody_looks(lens, past, bad, cache):
     """Infinities and NaN in slots behind the sequence and on unused pages; and in keys that only LATER tokens see."""
-    if cache == "e4m3" and bad == bad:
-        pytest.skip("e4m3 has no infinities")
     b = Batch(lens, past, 16, 4, 2, cache, seed=21)
     clean = {m: attn(b, m).clone() for m in (0, 1)}
     live = torch.zeros(b.num_pages, b.page, dtype=torch.bool)
@@ -259,11 +295,12 @@ def test_attention_same_bits_every_time(lens, past):
         assert torch.equal(attn(b, 1)[:b.T], first)
 
 
-def test_attention_far_pages():
-    """Pages whose offset passes 2^32 bytes."""
+@pytest.mark.parametrize("page", [16, 10])
+def test_far_pages(page):
+    """Pages whose offset passes 2^32 bytes, read and written."""
     if torch.cuda.mem_get_info()[0] < 50 << 30:
         pytest.skip("needs 50 GB")
-    b = Batch([1, 40], [70, 90], 16, 4, 2, seed=51)
+    b = Batch([1, 40], [70, 90], page, 4, 2, seed=51)
     far = (5 << 30) // 2 // 4                                # elements between pages: page 4 starts at 5 GiB
     far -= far % 8
     d = {n: getattr(b, n).to(DEV) for n in ("q", "table", "seq_start", "pos0", "kv_len")}
@@ -282,8 +319,23 @@ def test_attention_far_pages():
     stride, b.page_stride, pages, b.num_pages = b.page_stride, far, b.num_pages, spots
     got = attn(b, 1, dev=d)
     torch.cuda.synchronize()
-    b.page_stride, b.num_pages = stride, pages
     assert torch.equal(got, want)
+    # one new token on the page behind 2^32 bytes: only its slot changes
+    g = Batch([1], [0], page, 4, 2, seed=52)
+    g.table[0, 0], g.num_pages, g.page_stride = 4, spots, far
+    qkv, qw, kw = inputs(g)
+    cos, sin = rope(1)
+    near_b = Batch([1], [0], page, 4, 2, seed=52)
+    _, k_near, v_near = append(near_b, qkv, qw, kw, cos, sin)
+    before = pool_k[4 * far:].clone(), pool_v[4 * far:].clone()
+    d = {"k": pool_k, "v": pool_v, "table": g.table.to(DEV), "seq_start": g.seq_start.to(DEV), "pos0": g.pos0.to(DEV)}
+    append(g, qkv, qw, kw, cos, sin, dev=d, fetch=False)
+    for pool, old, new in ((pool_k, before[0], k_near), (pool_v, before[1], v_near)):
+        got = pool[4 * far:].view(2, page, D).cpu()
+        assert torch.equal(got[:, 0], near_b.pages(new)[int(near_b.table[0, 0]), :, 0])
+        assert torch.equal(got[:, 1:], old.view(2, page, D).cpu()[:, 1:])
+    assert not pool_k[:4 * far].view(4, far)[:, b.n_kv * page * D:].any()
+    b.page_stride, b.num_pages = stride, pages
 
 
 def test_attention_on_another_stream_and_in_a_graph():
@@ -312,7 +364,7 @@ def test_attention_on_another_stream_and_in_a_graph():
 
 
 # ------------------------------------------------------------------------------------------------ append
-def append(b, qkv, qw, kw, cos, sin, flags=0, in_place=False, eps=1e-6, dev=None):
+def append(b, qkv, qw, kw, cos, sin, flags=0, in_place=False, eps=1e-6, dev=None, fetch=True):
     d = dev or {n: getattr(b, n).to(DEV) for n in ("k", "v", "table", "seq_start", "pos0")}
     x = qkv.to(DEV).clone()
     q_out = x if in_place else torch.full((b.T, b.n_q * D + 16), float("nan"), device=DEV, dtype=BF)
@@ -325,7 +377,7 @@ def append(b, qkv, qw, kw, cos, sin, flags=0, in_place=False, eps=1e-6, dev=None
     torch.cuda.synchronize()
     if not in_place:
         assert torch.equal(x.cpu().view(torch.int16), qkv.view(torch.int16))
-    return q_out.cpu(), d["k"].cpu(), d["v"].cpu()
+    return (q_out.cpu(), d["k"].cpu(), d["v"].cpu()) if fetch else None
 
 
 def rope(n, theta=1e6):
@@ -420,6 +472,22 @@ def test_append_in_place_and_stepwise_bits():
         rows = x[5 * i:5 * i + 5]
         assert torch.equal(b.pages(k)[page_no, :, slot].reshape(5, -1), rows[:, 16 * D:24 * D])
         assert torch.equal(b.pages(v)[page_no, :, slot].reshape(5, -1), rows[:, 24 * D:32 * D])
+
+
+def test_append_thousands_of_sequences():
+    """Three steps of the search for a token's sequence; almost all sequences have no row."""
+    B = 5000
+    lens = [1 if i % 71 == 3 else 0 for i in range(B)]
+    b = Batch(lens, [i % 5 for i in range(B)], 4, 2, 1, seed=12)
+    qkv, qw, kw = inputs(b)
+    cos, sin = rope(8)
+    q_out, k, v = append(b, qkv, qw, kw, cos, sin)
+    for i in [i for i in range(B) if lens[i]]:
+        row, pos = b.starts[i], b.past[i]
+        x = qkv[row:row + 1, :4 * D].to(F64).view(1, 4, D)
+        q, mag = turned(x[:, :2], qw, cos[pos:pos + 1], sin[pos:pos + 1], 1e-6)
+        near(q_out[row:row + 1, :2 * D].view(1, 2, D), q, mag, BF)
+        assert torch.equal(b.pages(v)[int(b.table[i, pos // 4]), 0, pos % 4], qkv[row, 3 * D:4 * D])
 
 
 def test_append_skips_what_has_no_place():

@@ -67,6 +67,8 @@ def test_append_refuses(change, code, words):
     (dict(n_q=15), "SHAPE", "n_q"), (dict(max_kv=129), "SHAPE", "max_kv"), (dict(max_kv=-1), "SHAPE", "max_kv"),
     (dict(max_pages=0), "SHAPE", ""), (dict(ld_q=16 * 128 - 8), "SHAPE", "stride"), (dict(ld_out=16 * 128 - 8), "SHAPE", "stride"),
     (dict(scale=0.0), "ARG", "scale"), (dict(scale=-0.1), "ARG", "scale"), (dict(scale=NAN), "ARG", "scale"), (dict(scale=INF), "ARG", "scale"),
+    (dict(scale=1e-31), "ARG", "scale"), (dict(scale=1e20, cache_type=1, k_scale=1e20), "ARG", "k_scale"),
+    (dict(max_kv=(1 << 30) + 1, max_pages=1 << 27, ld_table=1 << 27), "SHAPE", "max_kv"),
     (dict(mask_block=-1), "ARG", "mask_block"), (dict(q=P + 8), "ALIGN", ""), (dict(ld_out=16 * 128 + 4), "ALIGN", ""),
     (dict(T=1 << 28), "SHAPE", "2^31"),
     # 4096 keys are more than one range: the workspace has to be there
