@@ -395,6 +395,8 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
                               long long ldc, int N, int K, void* workspace, long long workspace_bytes, void* stream) {
     const char* who = "coda_lora_bf16";
     if (B <= 0 || T <= 0 || n_adapters <= 0 || N <= 0 || K <= 0) return coda_refuse(who, CODA_ERR_SHAPE, "a size is not positive");
+    // running sums over 64 sequences of tiles stay below 2^31 even for starts that make every sequence T rows long
+    if (T > 1 << 28) return coda_refuse(who, CODA_ERR_SHAPE, "T exceeds 2^28");
     if (rank <= 0 || rank % 8 || rank > 128) return coda_refuse(who, CODA_ERR_SHAPE, "rank is a multiple of 8 up to 128");
     if (K % 64 || N % 8) return coda_refuse(who, CODA_ERR_SHAPE, "K % 64 or N % 8");
     if (ldx < K || ldr < N || ldc < N) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");

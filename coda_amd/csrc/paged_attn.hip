@@ -138,7 +138,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, TileRows&
             }
         }
         work = wave_sum(work);
-        range_keys = max(a.min_keys, ((int)fminf(work * a.per_range, 1e9f) + 128) & ~127);
+        range_keys = max(a.min_keys, ((int)fminf(work * a.per_range, 1.2e9f) + 128) & ~127);       // more than any kv_len: one range
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.range_keys = range_keys;
     }
     int k;
@@ -378,15 +378,13 @@ __device__ __forceinline__ bf16x8_t join4(s16x4_t a, s16x4_t b) {
 constexpr int FEW_TILE = 32;                                    // keys per tile
 constexpr int FEW_WAVE_LDS = FEW_TILE * 256;                    // V image, then 16 rows of fp32 output: 8 KiB a wave
 
-template <int RG, int RW, bool F8, bool G16>
-__global__ __launch_bounds__(256 * RW, RG == 1 && F8 ? 3 : 2) void paged_attn_few_kernel(AttnArgs a) {
+template <int RG, bool F8, bool G16>
+__global__ __launch_bounds__(256, RG == 1 && F8 ? 3 : 2) void paged_attn_few_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int R = 16 * RG * RW;
+    constexpr int R = 16 * RG;
     constexpr int NP = F8 ? 4 : 8;                              // 1 KiB pieces of a K or V tile
-    // weights as a bf16 pair (value and remainder): the second product per fragment hides under the page loads, and the weights keep
-    // 16 significant bits instead of 8
-    __shared__ float ml[4 * RW][2][16 * RG];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = wave & 3, rw = wave >> 2;
+    __shared__ float ml[4][2][16 * RG];
+    const int lane = threadIdx.x & 63, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, quad = lane >> 4;
     const int kvh = blockIdx.x % a.n_kv;
     TileRows tr;
@@ -436,14 +434,14 @@ __global__ __launch_bounds__(256 * RW, RG == 1 && F8 ? 3 : 2) void paged_attn_fe
     int lim[RG];
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-        const RowAt at = row_at(a, tr, kvh, min(tr.r0 + (rw * RG + rg) * 16 + c, tr.rows - 1));
+        const RowAt at = row_at(a, tr, kvh, min(tr.r0 + rg * 16 + c, tr.rows - 1));
         lim[rg] = limit_of(a, lm, at.token - tr.s0);
         const char* qp = a.q + (size_t)at.token * a.ldq_b + (size_t)at.head * 256;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) qf[rg][ks] = *(const bf16x8_t*)(qp + (F8 ? 8 * (ks >> 1) + 2 * quad + (ks & 1) : 4 * ks + quad) * 16);
     }
 
-    char* vimg = lds + wave * FEW_WAVE_LDS;
+    char* vimg = lds + kw * FEW_WAVE_LDS;
     f32x4_t o[RG][8];
     float m_run[RG], l_run[RG];
     unsigned int bad[RG];
@@ -530,7 +528,8 @@ __global__ __launch_bounds__(256 * RW, RG == 1 && F8 ? 3 : 2) void paged_attn_fe
                 }
             l_run[rg] += psum;
         }
-        // ---- O^T
+        // ---- O^T, the weights as a bf16 pair (value and remainder): the second product of each fragment hides under the page loads, and
+        // the weights keep 16 significant bits instead of 8
         bf16x8_t ph[RG], pl[RG];
 #pragma unroll
         for (int rg = 0; rg < RG; ++rg)
@@ -569,17 +568,16 @@ __global__ __launch_bounds__(256 * RW, RG == 1 && F8 ? 3 : 2) void paged_attn_fe
         float l = l_run[rg] + __shfl_xor(l_run[rg], 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (quad == 0) {
-            ml[wave][0][rg * 16 + c] = m_run[rg];
-            ml[wave][1][rg * 16 + c] = l;
+            ml[kw][0][rg * 16 + c] = m_run[rg];
+            ml[kw][1][rg * 16 + c] = l;
         }
     }
     __syncthreads();
-    const int w0 = rw * 4;                                      // first of this row wave's four
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-        float m = ml[w0][0][rg * 16 + c];
+        float m = ml[0][0][rg * 16 + c];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w0 + w][0][rg * 16 + c]);
+        for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][0][rg * 16 + c]);
         const float f = part_weight(m_run[rg], m);
         // a wave's own image region holds its 16 x 128 fp32 block: 16-byte chunk ch of row r at ch ^ r
         if (rg > 0) __syncthreads();                            // the block of the previous row group has been read
@@ -587,18 +585,18 @@ __global__ __launch_bounds__(256 * RW, RG == 1 && F8 ? 3 : 2) void paged_attn_fe
         for (int dt = 0; dt < 8; ++dt) *(f32x4_t*)(vimg + c * 512 + (((4 * dt + quad) ^ c) << 4)) = o[rg][dt] * f;
         __syncthreads();
         // key wave w joins rows 4 w .. 4 w + 3: lane -> row, 8 features
-        const int rr = kw * 4 + quad, tile_row = tr.r0 + (rw * RG + rg) * 16 + rr;
-        float acc[8], ll = 0.f, mm = ml[w0][0][rg * 16 + rr];
+        const int rr = kw * 4 + quad, tile_row = tr.r0 + rg * 16 + rr;
+        float acc[8], ll = 0.f, mm = ml[0][0][rg * 16 + rr];
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = 0.f;
 #pragma unroll
-        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, ml[w0 + w][0][rg * 16 + rr]);
+        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, ml[w][0][rg * 16 + rr]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            ll += ml[w0 + w][1][rg * 16 + rr] * part_weight(ml[w0 + w][0][rg * 16 + rr], mm);
+            ll += ml[w][1][rg * 16 + rr] * part_weight(ml[w][0][rg * 16 + rr], mm);
 #pragma unroll
             for (int q4 = 0; q4 < 2; ++q4) {
-                const f32x4_t x = *(const f32x4_t*)(lds + (w0 + w) * FEW_WAVE_LDS + rr * 512 + (((2 * c + q4) ^ rr) << 4));
+                const f32x4_t x = *(const f32x4_t*)(lds + w * FEW_WAVE_LDS + rr * 512 + (((2 * c + q4) ^ rr) << 4));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[4 * q4 + j] += x[j];
             }
@@ -974,13 +972,29 @@ Plan make_plan(int T, int B, int max_kv, int n_q, int n_kv, int cus) {
     const int g = n_q / n_kv;
     const double rho = (double)T * g / B;                       // rows per sequence and key/value head, on average
     Plan p;
-    p.R = rho <= 16 ? 16 : rho <= 32 ? 32 : rho <= 64 ? 64 : rho <= 128 ? 128 : 256;
+    // tiles per key/value head, at least, where no sequence is empty
+    auto tiles = [&](int R) {
+        const long long t = ((long long)T * g + R - 1) / R;
+        return t > B ? t : B;
+    };
+    const long long two = 2LL * cus;                            // workgroups of 256 threads that are resident at once
+    // us with tiles of so many rows, 16 heads on 8, bf16:
+    //   16 / 32      32 sequences x 2000 keys: rho 8 51 / 53, rho 16 51 / 53, rho 24 57 / 53
+    //   32 / 128     32 x 1000: rho 48 37 / 41, rho 64 40 / 45, rho 80 59 / 47; 128 x 1500: 183 / 216, 185 / 167, 246 / 176; 8 x 4000:
+    //                48 / 42, 49 / 44, 62 / 45; all tiles resident and keys short, 8 x 300: rho 64 13.7 / 16.7, rho 128 14.5 / 17.7
+    //   128 / 256    16 x 2000: rho 256 73 / 84; 4 x 1000: rho 768 50 / 48, rho 1024 55 / 63; 8 x 2048 new: 327 / 306, 2 x 8192 new 1209 /
+    //                1115, behind 8000 keys 1 x 1000 123 / 110, but 1 x 2048 new 72 / 79 (too few tiles for the chip)
+    // (64 rows on eight waves lost to 32 or 128 everywhere.)
+    if (rho <= 16) p.R = 16;
+    else if (rho <= 64 || (rho <= 128 && max_kv < 2048 && tiles(32) * n_kv <= two)) p.R = 32;
+    else p.R = rho > 1536 && tiles(256) * n_kv * (max_kv < 2048 ? 1 : max_kv / 2048) >= cus ? 256 : 128;
     const long long bound = (long long)T * g / p.R + B;         // tiles per key/value head, at most
-    const long long some = ((long long)T * g + p.R - 1) / p.R > B ? ((long long)T * g + p.R - 1) / p.R : B;   // and where no sequence is empty, at least
-    const long long slots = (p.R <= 32 || p.R == 128 ? 2 : 1) * (long long)cus;          // workgroups resident at once
-    // no range under eight steps of a workgroup (the second kernel and a short range's start cost as much), and no more partial outputs
-    // than 64 MiB
-    const int least = p.R <= 64 ? 1024 : 512;
+    const long long some = tiles(p.R);
+    const long long slots = p.R == 256 ? cus : two;
+    // no range under eight steps of a workgroup, 1024 or 512 keys (us at half / at it / at twice: 32 single tokens x 2000 keys 53.9 / 50.6 /
+    // 50.9, 4 x 20000 65.5 / 64.8 / 83.8; 8 blocks of 128 tokens x 2000 49.8 / 48.5 / 57.3, 8 of 200 x 4000 108 / 101 / 102), and no more
+    // partial outputs than 64 MiB
+    const int least = p.R <= 32 ? 1024 : 512;
     const long long row_bytes = (long long)T * n_q * (HEAD_DIM + 2) * 4;
     long long most = max_kv / least;
     if (most > (64LL << 20) / row_bytes) most = (64LL << 20) / row_bytes;
@@ -1015,6 +1029,8 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     const char* who = "coda_paged_attn";
     if (B <= 0 || T <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv) return coda_refuse(who, CODA_ERR_SHAPE, "a size is not positive, or n_q % n_kv");
     if ((long long)T * n_q > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "T * n_q exceeds 2^31 - 1");
+    // running sums over 64 sequences of tiles stay below 2^31 even for starts that make every sequence T rows long
+    if ((long long)T * (n_q / n_kv) > 1 << 28) return coda_refuse(who, CODA_ERR_SHAPE, "T * n_q / n_kv exceeds 2^28");
     if (max_kv < 0 || (long long)max_kv > (long long)max_pages * page_size || max_kv > 1 << 30)
         return coda_refuse(who, CODA_ERR_SHAPE, "max_kv is not within max_pages * page_size and 2^30");
     if (ld_q < (long long)n_q * HEAD_DIM || ld_out < (long long)n_q * HEAD_DIM) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");
@@ -1056,9 +1072,8 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     // pages of a multiple of 16 keys take the kernels that address 16 keys at a time
     auto pick = [&](auto f8c, auto g16c) -> int {
         constexpr bool F8 = decltype(f8c)::value, G16 = decltype(g16c)::value;
-        if (p.R == 16) return go(paged_attn_few_kernel<1, 1, F8, G16>, 256, 4 * FEW_WAVE_LDS);
-        if (p.R == 32) return go(paged_attn_few_kernel<2, 1, F8, G16>, 256, 4 * FEW_WAVE_LDS);
-        if (p.R == 64) return go(paged_attn_few_kernel<2, 2, F8, G16>, 512, 8 * FEW_WAVE_LDS);
+        if (p.R == 16) return go(paged_attn_few_kernel<1, F8, G16>, 256, 4 * FEW_WAVE_LDS);
+        if (p.R == 32) return go(paged_attn_few_kernel<2, F8, G16>, 256, 4 * FEW_WAVE_LDS);
         if (p.R == 128) return go(paged_attn_many_kernel<4, F8, G16>, 256, 2 * MANY_BUF);
         return go(paged_attn_many_kernel<8, F8, G16>, 512, 2 * MANY_BUF);
     };
@@ -1075,7 +1090,6 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     };
     if (p.R == 16) join(std::integral_constant<int, 16>{});
     else if (p.R == 32) join(std::integral_constant<int, 32>{});
-    else if (p.R == 64) join(std::integral_constant<int, 64>{});
     else if (p.R == 128) join(std::integral_constant<int, 128>{});
     else join(std::integral_constant<int, 256>{});
     CODA_CHECK_LAUNCH("paged_attn join");

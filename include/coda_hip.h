@@ -241,7 +241,7 @@ int coda_origin_transfer(long long* x, const long long* x0, const int* dst_pos, 
  * different lengths, or one denoise block behind a prefix that is kept.
  *
  * Batch.  T packed token rows; sequence b < B owns rows seq_start[b] .. seq_start[b+1]-1 (seq_start int32 [B+1] on the
- * device, not decreasing, within [0, T]; a sequence may have no row).  Rows of no sequence are neither read nor written.
+ * device, not decreasing, within [0, T]; a sequence may have no row).  Rows of no sequence are not written.
  * Cache.  k_cache / v_cache: pages [num_pages][n_kv][page_size][128], page_stride ELEMENTS from page to page (at least
  * n_kv * page_size * 128), both of the same geometry; page_size is any positive number.  Position p of sequence b lives in slot
  * p % page_size of page page_table[b * ld_table + p / page_size] (int32 on the device, max_pages entries a sequence).  An
@@ -271,11 +271,12 @@ int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out, long long 
  * sequence (decode) to whole prompts.  q and out bf16 [T, n_q * 128] (out apart from q and the cache).  Sequence b has
  * kv_len[b] keys, positions 0 .. kv_len[b]-1 (int32 [B]).  mask_block 0: a token sees all of them, later positions included
  * (the denoiser's attention).  mask_block m > 0: token i sees the keys before the end of its block of m positions,
- * j < ((pos0[b] + i) / m + 1) * m (1: causal).  A token that sees no key gets zeros.  Keys a token does not see
- * have no influence on it, whatever their slots hold; an infinity or NaN that it does see makes its output non-finite.
+ * j < ((pos0[b] + i) / m + 1) * m (1: causal).  A token that sees no key, or only scores of -infinity, gets zeros.  Keys a token
+ * does not see have no influence on it, whatever their slots hold; a NaN score or an infinity or NaN in V that it does see makes
+ * its output (of the feature, for V) non-finite.
  * max_kv: host-side bound of kv_len, at most max_pages * page_size and 2^30 (keys from max_kv on are not seen): it sizes the launch.
  * Scores, maxima, sums and outputs are fp32; weights enter the second product as bf16 (a bf16 pair where there are at most 64
- * rows per sequence and key/value head).  scale > 0, and scale * 1.4427 (e4m3: * k_scale) within [1e-30, 1e30].
+ * rows per sequence and key/value head).  T * n_q / n_kv is at most 2^28.  scale > 0, and scale * 1.4427 (e4m3: * k_scale) within [1e-30, 1e30].
  * workspace: coda_paged_attn_workspace_bytes(T, B, max_kv, n_q, n_kv) bytes (may be 0), 16-byte aligned, contents irrelevant before
  * and after; calls that may run at the same time need one each. */
 long long coda_paged_attn_workspace_bytes(int T, int B, int max_kv, int n_q, int n_kv);
@@ -290,7 +291,7 @@ int coda_paged_attn(const void* q, long long ld_q, void* out, long long ld_out, 
  * X bf16 [T, K] (the projection's input), R bf16 [T, N] (its output, e.g. of coda_gemm_bf16 CODA_EPI_PLAIN), C bf16 [T, N]: R
  * itself (in place) or memory apart from R and X.  A bf16 [n_adapters, rank, K], B bf16 [n_adapters, N, rank], both dense; scale
  * fp32 [n_adapters] on the device or NULL (1); adapter int32 [B], a value outside [0, n_adapters) means none: C[t] = R[t].
- * rank is a multiple of 8 up to 128 (adapters of smaller rank: zero rows of A), K % 64 == 0, N % 8 == 0.  Both products are summed in
+ * rank is a multiple of 8 up to 128 (adapters of smaller rank: zero rows of A), K % 64 == 0, N % 8 == 0, T at most 2^28.  Both products are summed in
  * fp32 and the result is rounded once; X A^T enters the second one as a bf16 pair (16 significant bits).
  * workspace: coda_lora_workspace_bytes(T, B, N, K, rank) bytes, 16-byte aligned, contents irrelevant before and after; calls
  * that may run at the same time need one each. */

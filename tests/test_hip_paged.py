@@ -143,7 +143,7 @@ def check(out, b, **kw):
     ([1, 1, 1], [31, 32, 200], 16, 8),                      # single tokens around a tile's edge
     ([0, 5, 0, 1, 0], [3, 60, 0, 127, 9], 6, 2),            # sequences without a row, g = 3
     ([32, 32], [96, 17], 16, 8),                            # denoise blocks: 64 rows
-    ([40, 3], [0, 300], 16, 8),                             # 80 rows: the four-wave tile
+    ([40, 3], [0, 300], 16, 8),                             # two tiles of 32 rows and a partial one
     ([130, 1, 77], [5, 64, 0], 16, 8),                      # past 128 rows, partial tiles
     ([300], [129], 12, 4),
 ])
@@ -172,6 +172,34 @@ def test_attention_ranges_of_keys(lens, past, cache):
         check(attn(b, mask), b, mask=mask)
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("page", [16, 10])
+@pytest.mark.parametrize("lens,past,n_q,n_kv,max_kv", [
+    ([200], [500], 320, 40, 700),                           # many heads: tiles enough without ranges
+    ([60, 40], [3000, 20], 64, 2, 40000),                   # few: ranges of keys, out of a long bound
+])
+def test_attention_widest_tiles(lens, past, n_q, n_kv, max_kv, page, cache):
+    """More than 1536 rows a sequence and key/value head: 256-row tiles."""
+    b = Batch(lens, past, page, n_q, n_kv, cache, seed=6, spare_rows=1)
+    pages = -(-max_kv // page)
+    b.table = torch.cat((b.table, torch.full((b.B, pages), -1, dtype=torch.int32)), 1)
+    b.max_pages += pages
+    assert (_lib.load().coda_paged_attn_workspace_bytes(b.T, b.B, max_kv, n_q, n_kv) > 0) == (n_kv == 2)
+    for mask in (0, 1, 32):
+        check(attn(b, mask, max_kv=max_kv), b, mask=mask)
+    # NaN in the last key's V, which under the causal mask only the last token sees
+    last = b.total[0] - 1
+    clean = attn(b, 1, max_kv=max_kv).clone()
+    v = b.pages(b.v.view(torch.uint8) if b.f8 else b.v.view(torch.int16))
+    v[int(b.table[0, last // page]), 0, last % page, 77] = 0x7f if b.f8 else torch.tensor(float("nan"), dtype=BF).view(torch.int16)
+    out, row = attn(b, 1, max_kv=max_kv), b.starts[1] - 1
+    hit = torch.zeros(b.T, n_q, D, dtype=torch.bool, device=DEV)
+    hit[row, :n_q // n_kv, 77] = True
+    hit = hit.view(b.T, -1)
+    hit[b.starts[-1]:] = True                               # rows of no sequence: never written
+    assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], clean[~hit])
+
+
 @pytest.mark.parametrize("B,past", [(150, 40), (300, 40), (300, 3000)])
 def test_attention_many_sequences(B, past):
     """More sequences than one step of the search covers, many of them without a row; the last case cuts the keys into ranges."""
@@ -181,7 +209,7 @@ def test_attention_many_sequences(B, past):
         check(attn(b, mask), b, mask=mask)
 
 
-@pytest.mark.parametrize("lens", [[1, 1, 1], [40, 3, 20], [70, 9, 9]])
+@pytest.mark.parametrize("lens", [[1, 1, 1], [40, 3, 20], [70, 9, 9], [200, 90, 30]])
 def test_attention_no_keys_beside_many(lens):
     """Ranges of keys, and sequences of the same call with none, one or no page."""
     b = Batch(lens, [4000, 10, 900], 16, 4, 2, seed=13)
@@ -219,7 +247,7 @@ def test_attention_starts_that_make_no_sense(starts):
 
 
 @pytest.mark.parametrize("page", [16, 10])
-@pytest.mark.parametrize("lens", [[1, 1], [30, 2], [60, 64], [150, 9]])
+@pytest.mark.parametrize("lens", [[1, 1], [30, 2], [60, 64], [150, 9], [90, 200]])
 def test_attention_lengths_and_bad_pages(lens, page):
     """kv_len of zero, negative or beyond max_kv; page numbers that are no pages.  A row that sees nothing gets zeros."""
     b = Batch(lens, [100, 100], page, 4, 2, seed=11)
@@ -245,7 +273,8 @@ def test_attention_lengths_and_bad_pages(lens, page):
 
 
 @pytest.mark.parametrize("cache,bad", [("bf16", float("inf")), ("bf16", float("-inf")), ("bf16", float("nan")), ("e4m3", float("nan"))])
-@pytest.mark.parametrize("lens,past", [([3], [40]), ([20, 9], [64, 10]), ([32, 30], [40, 41]), ([60, 2], [13, 90]), ([140], [77])])
+@pytest.mark.parametrize("lens,past", [([3], [40]), ([20, 9], [64, 10]), ([32, 30], [40, 41]), ([60, 2], [13, 90]), ([140], [77]),
+                                       ([90, 200], [13, 41])])
 def test_attention_nonfinite_where_nobody_looks(lens, past, bad, cache):
     """Infinities and NaN in slots behind the sequence and on unused pages; and in keys that only LATER tokens see."""
     b = Batch(lens, past, 16, 4, 2, cache, seed=21)

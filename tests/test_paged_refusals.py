@@ -70,7 +70,7 @@ def test_append_refuses(change, code, words):
     (dict(scale=1e-31), "ARG", "scale"), (dict(scale=1e20, cache_type=1, k_scale=1e20), "ARG", "k_scale"),
     (dict(max_kv=(1 << 30) + 1, max_pages=1 << 27, ld_table=1 << 27), "SHAPE", "max_kv"),
     (dict(mask_block=-1), "ARG", "mask_block"), (dict(q=P + 8), "ALIGN", ""), (dict(ld_out=16 * 128 + 4), "ALIGN", ""),
-    (dict(T=1 << 28), "SHAPE", "2^31"),
+    (dict(T=1 << 28), "SHAPE", "2^31"), (dict(T=(1 << 27) + 1, n_q=8, n_kv=4), "SHAPE", "2^28"),
     # 4096 keys are more than one range: the workspace has to be there
     (dict(max_kv=4096, max_pages=256, ld_table=256, workspace_bytes=1024), "ARG", "workspace"),
     (dict(max_kv=4096, max_pages=256, ld_table=256, workspace=None), "ARG", "workspace"),
@@ -97,7 +97,7 @@ LORA = dict(X=P, ldx=256, A=P, Bw=P, scale=None, seq_start=P, adapter=P, B=2, T=
 
 @pytest.mark.parametrize("change,code,words", [
     (dict(B=0), "SHAPE", "positive"), (dict(T=0), "SHAPE", "positive"), (dict(T=-3), "SHAPE", "positive"), (dict(n_adapters=0), "SHAPE", "positive"),
-    (dict(N=0), "SHAPE", "positive"), (dict(K=0), "SHAPE", "positive"), (dict(rank=0), "SHAPE", "rank"), (dict(rank=12), "SHAPE", "rank"),
+    (dict(T=(1 << 28) + 1), "SHAPE", "2^28"), (dict(N=0), "SHAPE", "positive"), (dict(K=0), "SHAPE", "positive"), (dict(rank=0), "SHAPE", "rank"), (dict(rank=12), "SHAPE", "rank"),
     (dict(rank=136), "SHAPE", "rank"), (dict(K=224), "SHAPE", "K % 64"), (dict(N=508), "SHAPE", "N % 8"), (dict(ldx=248), "SHAPE", "stride"),
     (dict(ldr=504), "SHAPE", "stride"), (dict(ldc=504), "SHAPE", "stride"),
     *[(dict([(n, None)]), "ARG", "null") for n in ("X", "A", "Bw", "seq_start", "adapter", "R", "C")],
