@@ -2,15 +2,18 @@
 //
 //     C[t] = R[t] + s[a] (X[t] A[a]^T) B[a]^T,     a = the adapter of t's sequence;  no adapter: C[t] = R[t]
 //
-// Two launches (one for small batches, lora_one_kernel).  `down` computes U = X A^T for tiles of one sequence's tokens, K cut over the waves of a workgroup and, where there
-// are few tiles, over workgroups (fp32 slabs in the workspace, summed in a fixed order by their readers).  `up` sums the slabs, scales, and
-// adds U B^T to R with R as the start value of the accumulators, so that the result is rounded once.
+// Two launches (one for small batches, lora_one_kernel).  `down` computes U = X A^T for tiles of one sequence's tokens, K cut over the
+// waves of a workgroup and, where there are few tiles, over workgroups (fp32 slabs in the workspace, summed in a fixed order by their
+// readers).  `up` sums the slabs, scales, computes U B^T in fp32 and adds R to it, so that the result is rounded once.
 //
 // v_mfma_f32_16x16x32_bf16 in both, weights as the A operand: a lane then holds four consecutive outputs (ranks, features) of one
 // token.  Both are bound by memory at serving ranks (8 .. 128).  X, A, R and C move as contiguous 512 bytes of a row, through LDS:
 // fragments straight from memory (16 rows x 64 B an instruction) took 27 + 120 us where this takes 22 + 95 (15.5 k tokens, rank 32,
 // 2048 -> 6144).  U enters the second product as a bf16 pair (value and remainder): the extra matrix instructions are free in a
 // kernel that waits for memory, and U keeps 16 bits.
+// Measured: 15.5 k tokens of 32 sequences, rank 32, 2048 -> 6144: down 22 us, up 91, together 517 MB at 4.6 TB/s (a large copy: 5.2); 32
+// blocks of 32 tokens, rank 64, 6144 -> 2048: 8 + 13 us, bound by the latency of one tile's chain; 32 single tokens, rank 16, 2048 ->
+// 4096, in one launch: 6.7 us.
 #include "paged_common.h"
 #include <type_traits>
 
@@ -21,7 +24,7 @@ namespace {
 struct Tile {
     int row0, n;                                // first token row, tokens (0: there is no such tile)
     int adapter;                                // -1: none
-    int unused;
+    int pad;                                    // 16 bytes each
 };
 
 struct LoraArgs {
@@ -139,12 +142,18 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
     const Tile t = a.tiles[slot];
     if (t.n == 0) return;
     const int col = lane & 15, quad = lane >> 4;
+    const int lr = threadIdx.x >> 5, lc = threadIdx.x & 31;     // row (of 8) and 16-byte chunk of a pass over 256 features
     if (t.adapter < 0) {
         if (a.r == a.c && a.ldr_b == a.ldc_b) return;
-        for (int m = 0; m < t.n; ++m) {
-            const size_t row = t.row0 + m;
-            for (int f = n0 + 8 * (int)threadIdx.x; f < n1; f += 2048)
-                *(u32x4_t*)(a.c + row * a.ldc_b + (size_t)f * 2) = *(const u32x4_t*)(a.r + row * a.ldr_b + (size_t)f * 2);
+        for (int f0 = n0; f0 < n1; f0 += 256) {                 // all rows of a step in flight: row after row took twice the kernel's time
+            u32x4_t v[2 * MT];
+            const int f = f0 + 8 * lc;
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+                v[i] = *(const u32x4_t*)(a.r + (size_t)(t.row0 + min(8 * i + lr, t.n - 1)) * a.ldr_b + (size_t)min(f, a.N - 8) * 2);
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+                if (8 * i + lr < t.n && f < n1) *(u32x4_t*)(a.c + (size_t)(t.row0 + 8 * i + lr) * a.ldc_b + (size_t)f * 2) = v[i];
         }
         return;
     }
@@ -154,7 +163,6 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
     __shared__ __attribute__((aligned(16))) char delta[16 * MT * 1024];
     bf16x8_t w[4][KS];
     u32x4_t rr[2 * MT];
-    const int lr = threadIdx.x >> 5, lc = threadIdx.x & 31;
     auto load = [&](int f0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

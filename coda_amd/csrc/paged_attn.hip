@@ -10,15 +10,17 @@
 // key/value head (row r = token r / g, head r % g) and tiles are cut from those: one token of a g = 2 model is two rows of one
 // tile, a block of 32 tokens is 64.
 //
-// MFMA orientation (v_mfma_f32_32x32x16_bf16), as in flash_attn.hip: S^T[key][row] = K Q^T with K rows from LDS and Q^T in
-// registers, so a lane holds one row's scores and the accumulator registers are directly the B operand of
-// O^T[d][row] += V^T P^T, whose A operand is read from LDS with the transposing ds_read_b64_tr_b16.
+// Two kernels: `few` (16 or 32 rows a workgroup; waves share the KEYS) for single tokens and short blocks, `many` (128 or 256 rows; waves
+// share the ROWS) for longer ones; make_plan has the rule and what both sides of it measured.  Both compute S^T[key][row] = K Q^T, so
+// that a lane holds scores of one row and its accumulators are directly the B operand of O^T[d][row] += V^T P^T, whose A operand
+// is read from LDS with the transposing ds_read_b64_tr_b16.
 // LDS image of a K or V tile: 256 B a key (bf16 also for e4m3 pages: the conversion is exact), 16-byte chunk ch of key r at
 // ch ^ swz(r): free of bank conflicts for both kinds of read.
 //
-// Pages reach LDS through registers (global loads of the NEXT tile fly under the current tile's products): keys of a tile
-// may lie on different pages, e4m3 is converted on the way, and keys beyond the sequence or on an invalid page are zeroed
-// on the way, so that whatever their slots hold (infinities, NaN) cannot reach the sums through 0 * x.
+// Pages come in through registers (loads of the NEXT tile fly under the current tile's products): keys of a tile may lie on different
+// pages, e4m3 is converted on the way, scores of keys that a row does not see are replaced, and values of keys beyond the
+// sequence or on an invalid page are zeroed on the way to LDS, so that whatever their slots hold (infinities, NaN) cannot reach the
+// sums through 0 * x.
 #include "paged_common.h"
 #include <type_traits>
 
@@ -199,7 +201,8 @@ __device__ __forceinline__ size_t shfl_size(size_t v, int src) {
 // Pages of a multiple of 16 keys (G16): 16 aligned keys lie on one page, one after the other.  Lane l holds the offset of 16-key group
 // 64 w + l of window w (1024 keys), so a tile's groups come out by readlane as wave-uniform bases, their keys are whole contiguous
 // KiB at constant offsets from them, and most tiles cost no look-up at all.
-// Other page sizes: lane l holds the offset of key l of the tile.
+// Other page sizes: lane l holds the offset of key l of the tile.  On the same pages this takes a little longer: 9.8 us against 9.4 (one
+// token, 1000 keys), 72.7 against 70.6 (128 single tokens, 333 MB of e4m3), 219 against 217 (prompts).
 template <int KEYS, bool G16>
 struct PageSource {
     static constexpr int UNIT = G16 ? 16 : 1, SPAN = G16 ? 64 : KEYS;     // keys per lane, lanes per look-up
@@ -366,12 +369,14 @@ __device__ __forceinline__ bf16x8_t join4(s16x4_t a, s16x4_t b) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few rows: RW x RG groups of 16.  Four KEY waves per row wave take tiles of 32 keys in turn, each with its own V image, maximum, sum
-// and output; they meet once, at the end.  No barrier in the loop.
+// Few rows: RG groups of 16.  Four waves take tiles of 32 keys in turn, each with its own V image, maximum, sum and output; they meet
+// once, at the end.  No barrier in the loop.
 //
 // What bounds it: the bytes of the cache (decode), or the latency of one tile after the other (short sequences).  So the next tile's
 // pages are in flight under this one's products, K goes from memory straight into the A fragments of v_mfma_f32_16x16x32_bf16 (a
 // quarter-wave reads 64 B of a key, the fragments of a tile are whole lines) and only V passes LDS, for its transposition.
+// Measured (16 heads on 8, one token a sequence): 128 x 2000 keys bf16 181 us = 5.8 TB/s, 128 x 4000 e4m3 189 us = 5.6 TB/s, 1 x 100000 81 us =
+// 5.0 TB/s with its join; 32 blocks of 32 tokens behind 2000 keys 65 us = 4.3 TB/s.  A large copy reaches 5.2 TB/s.
 //   S^T[key][row]:  lane -> row lane & 15, keys 16 kt + 4 quad + i          (quad = lane >> 4)
 //   P^T as B:       k index (quad, j) is key 16 (j >> 2) + 4 quad + (j & 3): the accumulators as they are
 //   O^T[d][row]:    lane -> row lane & 15, features 16 dt + 4 quad + i
@@ -619,7 +624,12 @@ __global__ __launch_bounds__(256, RG == 1 && F8 ? 3 : 2) void paged_attn_few_ker
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Many rows: NW waves of 32 rows each share a double-buffered stream of 64-key tiles.
+// Many rows: NW waves of 32 rows each share a double-buffered stream of 64-key tiles, one barrier a tile.
+//
+// What bounds it: the chain products - maximum - exponentials - products of a wave, which the other wave of its SIMD only partly
+// covers.  Measured: 8 x 2048 tokens, 16 heads on 8, no mask 306 us = 900 TFLOP/s, causal 181 us; 2 x 8192 no mask 985 TFLOP/s, of the 1257
+// that a large matrix product reaches on this card.  Slower or no faster: the two halves of the workgroup one barrier apart (341 us),
+// the softmax of a tile beside the scores of the next (311), wave priorities around the products (316).
 constexpr int MANY_TILE = 64;
 constexpr int MANY_BUF = 2 * MANY_TILE * 256;                   // K and V image: 32 KiB
 
@@ -866,7 +876,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
 // ---------------------------------------------------------------------------------------------------------------------
 // Joins the key ranges of (token, head) rows.  R: rows per tile of the kernel that wrote the ranges (the rows of a tile have the same
 // number of ranges).  Up to FEW_RANGES ranges: a wave per row, every range's loads in flight at once; more: a workgroup per row, the
-// ranges shared out over its eight half-waves, which meet in LDS.
+// ranges shared out over its eight half-waves, which meet in LDS.  Bound by latency (sequence, its length, the parts: three dependent
+// loads) or by the parts' bytes: 4.8 us for 2048 rows, 11.5 for 16384 rows of up to 4 ranges (71.6 against 55.4 for the whole call
+// with a workgroup per row).
 constexpr int FEW_RANGES = 8;
 
 template <int R>
