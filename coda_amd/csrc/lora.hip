@@ -11,9 +11,9 @@
 // fragments straight from memory (16 rows x 64 B an instruction) took 27 + 120 us where this takes 22 + 95 (15.5 k tokens, rank 32,
 // 2048 -> 6144).  U enters the second product as a bf16 pair (value and remainder): the extra matrix instructions are free in a
 // kernel that waits for memory, and U keeps 16 bits.
-// Measured: 15.5 k tokens of 32 sequences, rank 32, 2048 -> 6144: down 22 us, up 91, together 517 MB at 4.6 TB/s (a large copy: 5.2); 32
-// blocks of 32 tokens, rank 64, 6144 -> 2048: 8 + 13 us, bound by the latency of one tile's chain; 32 single tokens, rank 16, 2048 ->
-// 4096, in one launch: 6.7 us.
+// Measured: 15.5 k tokens of 32 sequences, rank 32, 2048 -> 6144: down 22 us, up 81, together 517 MB at 5.0 TB/s (a large copy: 5.2); 32
+// blocks of 32 tokens, rank 64, 6144 -> 2048: 8.5 + 7 us, bound by the latency of one tile's chain (tile, slabs, products, result);
+// 32 single tokens, rank 16, 2048 -> 4096, in one launch: 6.7 us.
 #include "paged_common.h"
 #include <type_traits>
 
@@ -364,20 +364,22 @@ struct Plan {
 
 Plan make_plan(int T, int B, int N, int K, int rank, int cus) {
     Plan p;
-    // 16 tokens a tile where sequences have no more on average, else 32.  64 measured no faster in the first launch (24 us against 22, 17 k
-    // tokens, rank 32, 2048 -> 6144) and slower in the second (120 against 96: fewer workgroups fit a CU), 16 slower in both
+    // 16 tokens a tile where sequences have no more on average, else 32 (us with 16 / 32: 32 x 16 tokens, rank 64, 2048 -> 4096 13.2 / 14.5,
+    // 32 x 20 15.5 / 15.0, 32 x 32, 6144 -> 2048 16.7 / 16.0, prompts as above 118 / 103; 64 a tile: fewer workgroups fit a CU, 120 us for
+    // `up` where 32 then took 96)
     p.mt = (double)T / B <= 16 ? 1 : 2;
     p.nslots = (long long)T / (16 * p.mt) + B;
     const long long tiles = ((long long)T + 16 * p.mt - 1) / (16 * p.mt) > B ? ((long long)T + 16 * p.mt - 1) / (16 * p.mt) : B;
     // One launch where a CU gets at most one workgroup of it and the A that each of them reads is small: us a call one / two launches, rank 16,
-    // 2048 -> 4096: 8.3 / 11.0 with 64 single tokens (256 workgroups), 13.2 / 11.1 with 128; rank 16, 6144 -> 2048 (A of 98 k values): equal
+    // 2048 -> 4096: 9.3 / 12.4 with 32 single tokens, 9.6 / 12.4 with 64 (256 workgroups), 13.7 / 13.6 with 128; rank 16, 6144 -> 2048 (A of
+    // 98 k values): equal
     p.one = p.mt == 1 && rank <= 32 && (long long)rank * K <= 65536 && tiles * ((N + 1023) / 1024) <= cus;
-    // features of a workgroup: two steps where that leaves a workgroup per CU (U is put together once for both: 135 us against 143 on the
-    // same prompts, and four steps 138), else one
+    // features of a workgroup: two steps where that leaves a workgroup per CU (U is put together once for both: prompts 103 us against 110
+    // with one step, and 104 with four), else one (32 blocks as above 15.4 us, 16.3 with two)
     p.nslice = tiles * ((N + 511) / 512) >= cus ? 512 : 256;
     // K ranges: one workgroup per CU; up to four where the slabs of U, written once and read by every slice of the second launch, stay under
-    // an eighth of X, R and C (prompts as above: 25 -> 22 us with two ranges; 32 blocks of 32 tokens, rank 64, 6144 -> 2048: 22.4 us with the
-    // eight ranges of one workgroup per CU, 27.6 with sixteen).  No range under one step of the four waves.
+    // an eighth of X, R and C.  us with 1 / 2 / 4 / 8 / 16 ranges: prompts 108 / 103 / 105 / 115 / 148 (two taken), 32 blocks 34 / 24 / 18 / 16.3
+    // / 19 (eight taken), 64 x 64 tokens, rank 64, 2048 -> 4096 34 / 30.5 / 30.7 / 37 / 52.  No range under one step of the four waves.
     const long long slab = 4LL * rank * (1 + (N + p.nslice - 1) / p.nslice), most = (2LL * K + 4LL * N) / 8 / slab;
     long long ks = (4LL * cus + tiles - 1) / tiles;
     if (ks > most) ks = most;
