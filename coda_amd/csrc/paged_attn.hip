@@ -20,7 +20,7 @@
 // Pages come in through registers (loads of the NEXT tile fly under the current tile's products): keys of a tile may lie on different
 // pages, e4m3 is converted on the way, scores of keys that a row does not see are replaced, and values of keys beyond the
 // sequence or on an invalid page are zeroed on the way to LDS, so that whatever their slots hold (infinities, NaN) cannot reach the
-// sums through 0 * x.
+// sums through 0 * x.  Whole bf16 tiles of the `many` kernel need none of that and are copied to LDS directly.
 #include "paged_common.h"
 #include <type_traits>
 
@@ -627,9 +627,11 @@ __global__ __launch_bounds__(256, RG == 1 && F8 ? 3 : 2) void paged_attn_few_ker
 // Many rows: NW waves of 32 rows each share a double-buffered stream of 64-key tiles, one barrier a tile.
 //
 // What bounds it: the chain products - maximum - exponentials - products of a wave, which the other wave of its SIMD only partly
-// covers.  Measured: 8 x 2048 tokens, 16 heads on 8, no mask 306 us = 900 TFLOP/s, causal 181 us; 2 x 8192 no mask 985 TFLOP/s, of the 1257
-// that a large matrix product reaches on this card.  Slower or no faster: the two halves of the workgroup one barrier apart (341 us),
-// the softmax of a tile beside the scores of the next (311), wave priorities around the products (316).
+// covers, and the LDS reads of every fragment for only 32 rows.  Measured, 16 heads on 8: 8 x 2048 tokens, no mask 306 us = 900 TFLOP/s,
+// causal 175 us; 2 x 8192 no mask 993 TFLOP/s, of the 1257 that a large matrix product reaches on this card.  Whole bf16 tiles straight to
+// LDS instead of through registers: 8 x 2048 causal 184 / 191 us (one card, in turn), 8 x 200 behind 4000 keys 106 / 117, 16 x 64 behind
+// 2000 54.5 / 57.  Slower or no faster: the two halves of the workgroup one barrier apart (341 us for 8 x 2048 without mask), the softmax of a
+// tile beside the scores of the next (311), wave priorities around the products (316).
 constexpr int MANY_TILE = 64;
 constexpr int MANY_BUF = 2 * MANY_TILE * 256;                   // K and V image: 32 KiB
 
@@ -662,10 +664,17 @@ struct ImageReader {
     }
 };
 
+// 16 bytes a lane, from a uniform base and a lane's offset, straight to a uniform LDS address + 16 lane; vmcnt counts it.  In asm because
+// the compiler waits for a copy that it knows of before every transposing read, which ends the overlap half a tile early.
+__device__ __forceinline__ void to_lds(const char* base, unsigned int in, unsigned int to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(in), "s"(base) : "m0", "memory");
+}
+
 template <int NW, bool F8, bool G16>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int R = 32 * NW;
+    constexpr bool DMA = !F8 && G16;
     constexpr int NP = (F8 ? 8 : 16) / NW;                      // 1 KiB pieces of a K (or V) tile per wave
     __shared__ int dropped_s[4];                                // tile t & 3: non-finite values were dropped from its V image
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -708,9 +717,25 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
 
     u32x4_t kr[NP], vr[NP];
     PageSource<MANY_TILE, G16> src;
-    auto fetch = [&](int t) {                                   // pieces i NW + wave of tile t; returns which of its keys exist
+    auto whole = [&](int t, unsigned long long ok) { return ok == ~0ull && k_lo + (t + 1) * MANY_TILE <= all; };
+    const unsigned int lds0 = (unsigned int)(uintptr_t)(CODA_LDS char*)lds;
+    // sends for pieces i NW + wave of tile t; returns which of its keys exist
+    auto send = [&](int t) {
         src.advance(a, table, k_lo, k_hi, t, 1);
+        const unsigned long long ok = src.exist(k_lo, k_hi, t);
         constexpr int ROW = F8 ? 128 : 256, PROWS = F8 ? 8 : 4, SUB = F8 ? 8 : 16;
+        if (DMA && whole(t, ok)) {
+            const unsigned int to = lds0 + (t & 1) * MANY_BUF;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int row = (i * NW + wave) * 4;
+                const size_t at = src.group(t, row >> 4) + (row & 15) * 256;
+                const unsigned int in = (lane >> 4) * 256 + (((lane & 15) ^ swz(row + (lane >> 4))) << 4);
+                to_lds(kbase + at, in, to + row * 256);
+                to_lds(vbase + at, in, to + MANY_TILE * 256 + row * 256);
+            }
+            return ok;
+        }
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int key = (i * NW + wave) * PROWS;
@@ -719,7 +744,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
             kr[i] = *(const u32x4_t*)(kbase + at + in);
             vr[i] = *(const u32x4_t*)(vbase + at + in);
         }
-        return src.exist(k_lo, k_hi, t);
+        return ok;
     };
     const ImageWriter<F8> img(lane);
     const ImageReader rd(lane);
@@ -788,11 +813,11 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
     if (threadIdx.x < 4) dropped_s[threadIdx.x] = 0;
     __syncthreads();
     if (nt > 0) {
-        // registers -> image of tile t; partly seen by the WORKGROUP's rows: it must hold finite values and zeros only
+        // tile t arrives in its image; partly seen by the WORKGROUP's rows: that must hold finite values and zeros only
         auto publish = [&](int t, unsigned long long ok) {
             char* kimg = lds + (t & 1) * MANY_BUF;
             char* vimg = kimg + MANY_TILE * 256;
-            if (ok != ~0ull || k_lo + (t + 1) * MANY_TILE > all) {
+            if (!whole(t, ok)) {
                 bool dropped = false;
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
@@ -800,6 +825,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
                     dropped |= img.template put<true>(vimg, i * NW + wave, vr[i], ok);
                 }
                 if (dropped) dropped_s[t & 3] = 1;
+            } else if (DMA) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             } else {
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
@@ -809,21 +836,15 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
             }
         };
         src.start(a, table, k_lo, k_hi, 0);
-        unsigned long long ok = fetch(0), ok_next = 0;
+        unsigned long long ok = send(0), ok_next = 0;
         publish(0, ok);
-        if (nt > 1) ok_next = fetch(1);
         for (int t = 0; t < nt; ++t) {
             // one barrier a tile: behind it tile t's image is complete and nobody reads tile t - 1's any more
             lds_barrier();
             const bool dropped = dropped_s[t & 3] != 0;
             if (threadIdx.x == 0) dropped_s[(t + 2) & 3] = 0;   // last read two barriers ago, next written behind the next one
-            unsigned long long ok_after = 0;
-            if (t + 1 < nt) {
-                publish(t + 1, ok_next);
-                __builtin_amdgcn_sched_barrier(0);
-                if (t + 2 < nt) ok_after = fetch(t + 2);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            if (t + 1 < nt) ok_next = send(t + 1);
+            __builtin_amdgcn_sched_barrier(0);
             const char* kimg = lds + (t & 1) * MANY_BUF;
             const int key0 = k_lo + t * MANY_TILE;
             if (key0 < w_any) {                                 // else none of this wave's rows sees the tile
@@ -832,8 +853,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
                     bad |= find_nonfinite<F8>(a, table, head_off, key0, MANY_TILE, k_hi, lim, 64,
                                               [&](int e) { return 32 * (e >> 4) + (e & 3) + 8 * ((e >> 2) & 3) + 4 * h; });
             }
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < nt) publish(t + 1, ok_next);
             ok = ok_next;
-            ok_next = ok_after;
         }
     }
 
