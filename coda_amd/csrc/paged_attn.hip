@@ -897,10 +897,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Joins the key ranges of (token, head) rows.  R: rows per tile of the kernel that wrote the ranges (the rows of a tile have the same
-// number of ranges).  Up to FEW_RANGES ranges: a wave per row, every range's loads in flight at once; more: a workgroup per row, the
-// ranges shared out over its eight half-waves, which meet in LDS.  Bound by latency (sequence, its length, the parts: three dependent
-// loads) or by the parts' bytes: 4.8 us for 2048 rows, 11.5 for 16384 rows of up to 4 ranges (71.6 against 55.4 for the whole call
-// with a workgroup per row).
+// number of ranges).  Up to FEW_RANGES ranges: half a wave per row, two heads of a token in a wave (one search), every range's loads in
+// flight at once; more: a workgroup per row, the ranges shared out over its eight half-waves, which meet in LDS.  Bound by latency
+// (sequence, its length, the parts: three dependent loads) or by the parts' bytes: 4.7 us for 2048 rows, 7.7 for 16384 rows of up to 4
+// ranges, where a wave per row took 11.1 and a workgroup per row 28.
 constexpr int FEW_RANGES = 8;
 
 template <int R>
@@ -916,33 +916,39 @@ __device__ __forceinline__ int ranges_of(const AttnArgs& a, int token, int head)
 
 template <int R>
 __global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int row = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
-    const int rows = a.T * a.n_q;
-    if (row >= rows) return;
-    const int token = row / a.n_q, head = row % a.n_q;
-    const int nsp = ranges_of<R>(a, token, head);
-    if (nsp <= 1) return;                                       // written by the first kernel
-    f32x2_t e[FEW_RANGES], x[FEW_RANGES];
+    const int lane = threadIdx.x & 63, l = lane & 31;
+    const int unit = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
+    const int pairs = (a.n_q + 1) / 2, token = unit / pairs;
+    if (token >= a.T) return;
+    const int head = unit % pairs * 2 + (lane >> 5);
+    int nsp = ranges_of<R>(a, token, head);
+    if (nsp <= 1 || head >= a.n_q) nsp = 0;                     // written by the first kernel
+    const size_t rows = (size_t)a.T * a.n_q, row = (size_t)token * a.n_q + min(head, a.n_q - 1);
+    f32x2_t e[FEW_RANGES];
+    f32x4_t x[FEW_RANGES];
 #pragma unroll
     for (int i = 0; i < FEW_RANGES; ++i) {
-        const size_t at = (size_t)min(i, nsp - 1) * rows + row;
+        if (!__any(i < nsp)) break;
+        const size_t at = (size_t)max(min(i, nsp - 1), 0) * rows + row;
         e[i] = *(const f32x2_t*)(a.pml + at * 2);
-        x[i] = *(const f32x2_t*)(a.po + at * HEAD_DIM + 2 * lane);
+        x[i] = *(const f32x4_t*)(a.po + at * HEAD_DIM + 4 * l);
     }
-    float mm = -INFINITY, tot = 0.f, y0 = 0.f, y1 = 0.f;
+    float mm = -INFINITY, tot = 0.f;
+    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < FEW_RANGES; ++i) mm = fmaxf(mm, e[i][0]);
+    for (int i = 0; i < FEW_RANGES; ++i)
+        if (i < nsp) mm = fmaxf(mm, e[i][0]);
 #pragma unroll
     for (int i = 0; i < FEW_RANGES; ++i) {
         if (i >= nsp) break;
         const float f = part_weight(e[i][0], mm);
         tot += e[i][1] * f;
-        y0 += x[i][0] * f;
-        y1 += x[i][1] * f;
+        y = y + x[i] * f;
     }
+    if (nsp == 0) return;
     const float inv = tot == 0.f ? 0.f : a.v_scale / tot;
-    *(unsigned int*)(a.out + (size_t)token * a.ldo_b + (size_t)head * 256 + lane * 4) = pack_bf16x2(y0 * inv, y1 * inv);
+    *(u32x2_t*)(a.out + (size_t)token * a.ldo_b + (size_t)head * 256 + l * 8) =
+        (u32x2_t){pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
 }
 
 template <int R>
@@ -1119,7 +1125,7 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     const long long rows = (long long)T * n_q;
     auto join = [&](auto tile_rows) {
         constexpr int R = decltype(tile_rows)::value;
-        if (p.max_ranges <= FEW_RANGES) hipLaunchKernelGGL(paged_attn_join_few_kernel<R>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+        if (p.max_ranges <= FEW_RANGES) hipLaunchKernelGGL(paged_attn_join_few_kernel<R>, dim3((unsigned)(((long long)T * ((n_q + 1) / 2) + 3) / 4)), dim3(256), 0, st, a);
         else hipLaunchKernelGGL(paged_attn_join_kernel<R>, dim3((unsigned)rows), dim3(256), 0, st, a);
     };
     if (p.R == 16) join(std::integral_constant<int, 16>{});
