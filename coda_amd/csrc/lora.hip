@@ -12,7 +12,7 @@
 // 2048 -> 6144).  U enters the second product as a bf16 pair (value and remainder): the extra matrix instructions are free in a
 // kernel that waits for memory, and U keeps 16 bits.
 // Measured: 15.5 k tokens of 32 sequences, rank 32, 2048 -> 6144: down 22 us, up 81, together 517 MB at 5.0 TB/s (a large copy: 5.2); 32
-// blocks of 32 tokens, rank 64, 6144 -> 2048: 8.5 + 7 us, bound by the latency of one tile's chain (tile, slabs, products, result);
+// blocks of 32 tokens, rank 64, 6144 -> 2048: 7.7 + 7 us, bound by the latency of one tile's chain (tile, slabs, products, result);
 // 32 single tokens, rank 16, 2048 -> 4096, in one launch: 6.7 us.
 #include "paged_common.h"
 #include <type_traits>
@@ -53,8 +53,8 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs& a, int slot) {
 }
 
 // U of 16 MT tokens, 16 RT ranks (those beyond the adapter's are computed from its last row and dropped).
-// Steps of 256 elements: rows of X and A come in as contiguous 512 bytes through registers (the next step's fly under this one's
-// products) into an LDS image, 16-byte chunk ch of row r at ch ^ (r & 15), and the four waves take 64 elements of each step.
+// Steps of 256 elements: rows of X and A come in as contiguous 512 bytes through registers (those of the next two steps fly under this
+// one's products: 7.7 us, one step ahead 8.4, 32 blocks of 32 tokens, rank 64, K 6144) into an LDS image, 16-byte chunk ch of row r at ch ^ (r & 15), and the four waves take 64 elements of each step.
 template <int MT, int RT>
 struct Down {
     static constexpr int ROWS = 16 * (MT + RT);
@@ -80,8 +80,8 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
                              : a.a + ((size_t)t.adapter * a.rank + min(r - 16 * MT, a.rank - 1)) * a.K * 2);
     }
     const int k0 = ks * a.kchunk, k1 = min(a.K, k0 + a.kchunk);
-    u32x4_t v[NL];
-    auto fetch = [&](int k) {
+    u32x4_t va[NL], vb[NL];
+    auto fetch = [&](u32x4_t (&v)[NL], int k) {
         const size_t at = (size_t)min(k + 8 * lc, a.K - 8) * 2; // past K: something that exists; the products stop at k1
 #pragma unroll
         for (int i = 0; i < NL; ++i) v[i] = *(const u32x4_t*)(src[i] + at);
@@ -92,12 +92,13 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[m][r] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     const int row = lane & 15, quad = lane >> 4;
-    fetch(k0);
-    for (int k = k0; k < k1; k += 256) {
+    fetch(va, k0);
+    if (k0 + 256 < k1) fetch(vb, k0 + 256);
+    auto step = [&](u32x4_t (&v)[NL], int k) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) *(u32x4_t*)(lds + (8 * i + lr) * 512 + ((lc ^ ((8 * i + lr) & 15)) << 4)) = v[i];
         __syncthreads();
-        if (k + 256 < k1) fetch(k + 256);
+        if (k + 512 < k1) fetch(v, k + 512);
         if (k + 64 * wave < k1) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -114,6 +115,10 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
             }
         }
         __syncthreads();
+    };
+    for (int k = k0; k < k1; k += 512) {
+        step(va, k);
+        if (k + 256 < k1) step(vb, k + 256);
     }
     f32x4_t* part = (f32x4_t*)lds;                              // [4][MT RT][64]
 #pragma unroll
