@@ -67,9 +67,14 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int NL = Down<MT, RT>::NL;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int slot = blockIdx.x / a.ksplit, ks = blockIdx.x % a.ksplit;
+    // Two workgroups share the ranks beyond 64, eight apart, so that they run on one XCD and find X in its L2.  (One with all 128 has a CU to
+    // itself and nothing to run beside its waits: 15.5 k tokens, rank 128, 6144 -> 2048 227 us against 196, 2048 -> 2048 137 against 123.)
+    const bool two = a.rank > 16 * RT;
+    const int half = two ? (blockIdx.x >> 3) & 1 : 0, unit = two ? (int)(blockIdx.x >> 4) * 8 + (int)(blockIdx.x & 7) : (int)blockIdx.x;
+    const int slot = unit / a.ksplit, ks = unit % a.ksplit, rank0 = half * 16 * RT;
+    if (slot >= a.nslots) return;
     const Tile t = find_tile<16 * MT>(a, slot);
-    if (ks == 0 && threadIdx.x == 0) a.tiles[slot] = t;
+    if (ks == 0 && half == 0 && threadIdx.x == 0) a.tiles[slot] = t;
     if (t.n == 0 || t.adapter < 0) return;
     const int lr = threadIdx.x >> 5, lc = threadIdx.x & 31;     // this thread's row (of 8) and chunk in a pass
     const char* src[NL];
@@ -77,7 +82,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     for (int i = 0; i < NL; ++i) {
         const int r = 8 * i + lr;
         src[i] = (i < 2 * MT ? a.x + (size_t)(t.row0 + min(r, t.n - 1)) * a.ldx_b
-                             : a.a + ((size_t)t.adapter * a.rank + min(r - 16 * MT, a.rank - 1)) * a.K * 2);
+                             : a.a + ((size_t)t.adapter * a.rank + min(rank0 + r - 16 * MT, a.rank - 1)) * a.K * 2);
     }
     const int k0 = ks * a.kchunk, k1 = min(a.K, k0 + a.kchunk);
     u32x4_t va[NL], vb[NL];
@@ -133,14 +138,15 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
         if (i >= MT * RT) break;
         const f32x4_t* p = part + i * 64 + lane;
         const f32x4_t sum = (p[0] + p[MT * RT * 64]) + (p[2 * MT * RT * 64] + p[3 * MT * RT * 64]);
-        const int tok = 16 * (i / RT) + row, r0 = 16 * (i % RT) + 4 * quad;
+        const int tok = 16 * (i / RT) + row, r0 = rank0 + 16 * (i % RT) + 4 * quad;
         if (tok < t.n && r0 < a.rank) *(f32x4_t*)(u + (size_t)(t.row0 + tok) * a.rank + r0) = sum;       // rank % 8 == 0
     }
 }
 
-// 16 MT tokens x nslice features; KS steps of 32 ranks
+// 16 MT tokens x nslice features; KS steps of 32 ranks.  Two workgroups a CU also at KS = 4, by the launch bound: rank 128 as in `down` 171 us
+// where one took 196; three or four at smaller KS spill (118 us against 103 at rank 32).
 template <int MT, int KS>
-__global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
+__global__ __launch_bounds__(256, 2) void lora_up_kernel(LoraArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nsl = (a.N + a.nslice - 1) / a.nslice;
     const int slot = blockIdx.x / nsl, n0 = (blockIdx.x % nsl) * a.nslice, n1 = min(a.N, n0 + a.nslice);
@@ -422,7 +428,7 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
     if (!p.one && (!workspace || workspace_bytes < plan_bytes(p, T, rank)))
         return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_lora_workspace_bytes");
     if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
-    const long long downs = p.nslots * p.ksplit, ups = p.nslots * ((N + p.nslice - 1) / p.nslice);
+    const long long downs = rank > 64 ? (p.nslots * p.ksplit + 7) / 8 * 16 : p.nslots * p.ksplit, ups = p.nslots * ((N + p.nslice - 1) / p.nslice);
     if (downs > 0x7fffffffLL || ups > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
     LoraArgs a;
     a.x = (const char*)X; a.ldx_b = ldx * 2;
@@ -455,8 +461,7 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
         int rc;
         if (rank <= 16) rc = down(lora_down_kernel<MT, 1>, Down<MT, 1>::LDS);
         else if (rank <= 32) rc = down(lora_down_kernel<MT, 2>, Down<MT, 2>::LDS);
-        else if (rank <= 64) rc = down(lora_down_kernel<MT, 4>, Down<MT, 4>::LDS);
-        else rc = down(lora_down_kernel<MT, 8>, Down<MT, 8>::LDS);
+        else rc = down(lora_down_kernel<MT, 4>, Down<MT, 4>::LDS);
         if (rc != CODA_OK) return rc;
         if (rank <= 32) hipLaunchKernelGGL((lora_up_kernel<MT, 1>), gu, block, 0, st, a);
         else if (rank <= 64) hipLaunchKernelGGL((lora_up_kernel<MT, 2>), gu, block, 0, st, a);
