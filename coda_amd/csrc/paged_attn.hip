@@ -627,11 +627,11 @@ __global__ __launch_bounds__(256, RG == 1 && F8 ? 3 : 2) void paged_attn_few_ker
 // Many rows: NW waves of 32 rows each share a double-buffered stream of 64-key tiles, one barrier a tile.
 //
 // What bounds it: the chain products - maximum - exponentials - products of a wave, which the other wave of its SIMD only partly
-// covers, and the LDS reads of every fragment for only 32 rows.  Measured, 16 heads on 8: 8 x 2048 tokens, no mask 306 us = 900 TFLOP/s,
-// causal 175 us; 2 x 8192 no mask 993 TFLOP/s, of the 1257 that a large matrix product reaches on this card.  Whole bf16 tiles straight to
-// LDS instead of through registers: 8 x 2048 causal 184 / 191 us (one card, in turn), 8 x 200 behind 4000 keys 106 / 117, 16 x 64 behind
-// 2000 54.5 / 57.  Slower or no faster: the two halves of the workgroup one barrier apart (341 us for 8 x 2048 without mask), the softmax of a
-// tile beside the scores of the next (311), wave priorities around the products (316).
+// covers, and the LDS reads of every fragment for only 32 rows.  Measured, 16 heads on 8: 8 x 2048 tokens, no mask 312 us = 880 TFLOP/s,
+// causal 184 us; 2 x 8192 no mask 1109 us = 991 TFLOP/s, of the 1257 that a large matrix product reaches on this card.  Whole bf16 tiles
+// straight to LDS instead of through registers: 8 x 2048 causal 184 / 191 us (one card, in turn), 8 x 200 behind 4000 keys 106 / 117, 16 x
+// 64 behind 2000 54.5 / 57.  Slower or no faster, against 303 .. 314 us for 8 x 2048 without mask through registers: the two halves of the
+// workgroup one barrier apart (341), the softmax of a tile beside the scores of the next (311), wave priorities around the products (316).
 constexpr int MANY_TILE = 64;
 constexpr int MANY_BUF = 2 * MANY_TILE * 256;                   // K and V image: 32 KiB
 
