@@ -163,3 +163,62 @@ def test_ragged_chunks_equal_whole_prompts(engine, page, cache, adapted):
     for b in range(4):
         # e4m3: a key that rounds the other way moves by a step of 2^-3, some of the time; averaged over the keys of a row
         assert rel(torch.cat(got[b]), whole[starts[b]:starts[b + 1]]) < (BAND if cache == _lib.CACHE_BF16 else 4 * BAND)
+
+
+def test_captured_step_replayed_over_growing_caches():
+    """Projection, adapters, append and attention of single tokens as one captured graph: replayed while the lengths on the device grow,
+    with eager work between the replays, against the same calls made one by one on their own caches."""
+    g = torch.Generator().manual_seed(6)
+    B, page, max_kv, rank, n_ad = 5, 16, 3000, 64, 3
+    max_pages = -(-max_kv // page)
+    rnd = lambda *shape, scale=1.0: (torch.randn(*shape, generator=g) * scale).to(BF).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    w, la, lb = rnd(QKV, H, scale=H ** -0.5), rnd(n_ad, rank, H, scale=H ** -0.5), rnd(n_ad, QKV, rank, scale=0.1)
+    qn, kn = rnd(D), rnd(D)
+    ang = torch.arange(max_kv)[:, None] / 1e6 ** (torch.arange(0, D, 2) / D)[None, :]
+    cos, sin = (f(torch.cat((ang, ang), -1)).to(BF).to(DEV) for f in (torch.cos, torch.sin))
+    table = torch.randperm(B * max_pages, generator=g).view(B, max_pages).to(torch.int32).to(DEV)
+    k0, v0 = rnd(B * max_pages, N_KV, page, D), rnd(B * max_pages, N_KV, page, D)
+    seq, pos0, kv, which = i32(list(range(B + 1))), i32([2900, 0, 15, 1000, 2047]), i32([0] * B), i32([0, 2, -1, 1, 0])
+    x = rnd(B, H)
+    lib = _lib.load()
+
+    class Side:
+        def __init__(self):
+            self.k, self.v = k0.clone(), v0.clone()
+            self.qkv, self.out = torch.empty(B, QKV, dtype=BF, device=DEV), torch.empty(B, N_Q * D, dtype=BF, device=DEV)
+            sizes = lib.coda_lora_workspace_bytes(B, B, QKV, H, rank), lib.coda_paged_attn_workspace_bytes(B, B, max_kv, N_Q, N_KV)
+            assert min(sizes) > 0                               # two launches each
+            self.ws = [torch.empty(n, dtype=torch.uint8, device=DEV) for n in sizes]
+
+        def enqueue(self):
+            s, qkv = _s(), self.qkv
+            _lib.call("coda_gemm_bf16", x.data_ptr(), H, None, w.data_ptr(), H, qkv.data_ptr(), QKV, None, 0, B, QKV, H, _lib.EPI_PLAIN, s)
+            _lib.call("coda_lora_bf16", x.data_ptr(), H, la.data_ptr(), lb.data_ptr(), None, seq.data_ptr(), which.data_ptr(), B, B, n_ad, rank,
+                      qkv.data_ptr(), QKV, qkv.data_ptr(), QKV, QKV, H, self.ws[0].data_ptr(), self.ws[0].numel(), s)
+            geo = (table.data_ptr(), max_pages, max_pages, self.k.data_ptr(), self.v.data_ptr(), N_KV * page * D, B * max_pages, page,
+                   _lib.CACHE_BF16, 1.0, 1.0)
+            _lib.call("coda_paged_append", qkv.data_ptr(), QKV, qkv.data_ptr(), QKV, qn.data_ptr(), kn.data_ptr(), cos.data_ptr(),
+                      sin.data_ptr(), max_kv, seq.data_ptr(), pos0.data_ptr(), B, B, *geo, N_Q, N_KV, 1e-6, 0, s)
+            _lib.call("coda_paged_attn", qkv.data_ptr(), QKV, self.out.data_ptr(), N_Q * D, seq.data_ptr(), pos0.data_ptr(), kv.data_ptr(), B, B,
+                      *geo, max_kv, N_Q, N_KV, 1 / math.sqrt(D), 1, self.ws[1].data_ptr(), self.ws[1].numel(), s)
+
+    kv.copy_(pos0 + 1)
+    eager, captured = Side(), Side()
+    captured.enqueue()                                          # first launches outside the capture; its caches are made anew
+    torch.cuda.synchronize()
+    captured.k.copy_(k0)
+    captured.v.copy_(v0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.enqueue()
+    for turn in range(4):
+        x.copy_(rnd(B, H))
+        kv.copy_(pos0 + 1)
+        graph.replay()
+        eager.enqueue()
+        torch.cuda.synchronize()
+        assert torch.isfinite(eager.out).all()
+        for a, b in ((captured.out, eager.out), (captured.k, eager.k), (captured.v, eager.v)):
+            assert torch.equal(a, b), turn
+        pos0 += 7                                               # also leaves slots that nobody wrote: those of the random cache
