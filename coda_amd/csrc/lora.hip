@@ -376,8 +376,8 @@ struct Plan {
 Plan make_plan(int T, int B, int N, int K, int rank, int cus) {
     Plan p;
     // 16 tokens a tile where sequences have no more on average, else 32 (us with 16 / 32: 32 x 16 tokens, rank 64, 2048 -> 4096 13.2 / 14.5,
-    // 32 x 20 15.5 / 15.0, 32 x 32, 6144 -> 2048 16.7 / 16.0, prompts as above 118 / 103; 64 a tile: fewer workgroups fit a CU, 120 us for
-    // `up` where 32 then took 96)
+    // 32 x 20 15.5 / 15.0, 32 x 32, 6144 -> 2048 16.7 / 16.0, prompts as above 118 / 103).  64 a tile, with fewer
+    // workgroups on a CU: prompts, rank 64, 6144 -> 2048 108 against 106, rank 128 184 against 171
     p.mt = (double)T / B <= 16 ? 1 : 2;
     p.nslots = (long long)T / (16 * p.mt) + B;
     const long long tiles = ((long long)T + 16 * p.mt - 1) / (16 * p.mt) > B ? ((long long)T + 16 * p.mt - 1) / (16 * p.mt) : B;
