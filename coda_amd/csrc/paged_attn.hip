@@ -897,11 +897,11 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Joins the key ranges of (token, head) rows.  R: rows per tile of the kernel that wrote the ranges (the rows of a tile have the same
-// number of ranges).  Up to FEW_RANGES ranges: half a wave per row, two heads of a token in a wave (one search), every range's loads in
-// flight at once; more: a workgroup per row, the ranges shared out over its eight half-waves, which meet in LDS.  Bound by latency
-// (sequence, its length, the parts: three dependent loads) or by the parts' bytes: 4.7 us for 2048 rows, 7.7 for 16384 rows of up to 4
-// ranges, where a wave per row took 11.1 and a workgroup per row 28.
-constexpr int FEW_RANGES = 8;
+// number of ranges).  `rows`: half a wave per row, two heads of a token in a wave (one search), the loads of eight ranges in flight at once.
+// `join`: a workgroup per row, the ranges shared out over its eight half-waves, which meet in LDS: for many ranges of few rows (us a call:
+// 16 rows of 47 ranges 17.1 / 15.6, 64 rows 24.3 / 22.5, but 1600 rows of 24 ranges 40.7 / 53.7).  Bound by latency (sequence, its
+// length, the parts: three dependent loads) or by the parts' bytes: 4.7 us for 2048 rows, 8.0 for 16384 rows of up to 4 ranges.
+constexpr int AT_ONCE = 8;
 
 template <int R>
 __device__ __forceinline__ int ranges_of(const AttnArgs& a, int token, int head) {
@@ -915,7 +915,7 @@ __device__ __forceinline__ int ranges_of(const AttnArgs& a, int token, int head)
 }
 
 template <int R>
-__global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void paged_attn_join_rows_kernel(AttnArgs a) {
     const int lane = threadIdx.x & 63, l = lane & 31;
     const int unit = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
     const int pairs = (a.n_q + 1) / 2, token = unit / pairs;
@@ -924,27 +924,36 @@ __global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
     int nsp = ranges_of<R>(a, token, head);
     if (nsp <= 1 || head >= a.n_q) nsp = 0;                     // written by the first kernel
     const size_t rows = (size_t)a.T * a.n_q, row = (size_t)token * a.n_q + min(head, a.n_q - 1);
-    f32x2_t e[FEW_RANGES];
-    f32x4_t x[FEW_RANGES];
-#pragma unroll
-    for (int i = 0; i < FEW_RANGES; ++i) {
-        if (!__any(i < nsp)) break;
-        const size_t at = (size_t)max(min(i, nsp - 1), 0) * rows + row;
-        e[i] = *(const f32x2_t*)(a.pml + at * 2);
-        x[i] = *(const f32x4_t*)(a.po + at * HEAD_DIM + 4 * l);
-    }
-    float mm = -INFINITY, tot = 0.f;
+    float m = -INFINITY, tot = 0.f;
     f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+    auto some = [&](int i0) {
+        f32x2_t e[AT_ONCE];
+        f32x4_t x[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < FEW_RANGES; ++i)
-        if (i < nsp) mm = fmaxf(mm, e[i][0]);
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (!__any(i0 + i < nsp)) break;
+            const size_t at = (size_t)max(min(i0 + i, nsp - 1), 0) * rows + row;
+            e[i] = *(const f32x2_t*)(a.pml + at * 2);
+            x[i] = *(const f32x4_t*)(a.po + at * HEAD_DIM + 4 * l);
+        }
+        float mn = m;
 #pragma unroll
-    for (int i = 0; i < FEW_RANGES; ++i) {
-        if (i >= nsp) break;
-        const float f = part_weight(e[i][0], mm);
-        tot += e[i][1] * f;
-        y = y + x[i] * f;
-    }
+        for (int i = 0; i < AT_ONCE; ++i)
+            if (i0 + i < nsp) mn = fmaxf(mn, e[i][0]);
+        const float fo = part_weight(m, mn);
+        tot *= fo;
+        y = y * fo;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (i0 + i >= nsp) break;
+            const float f = part_weight(e[i][0], mn);
+            tot += e[i][1] * f;
+            y = y + x[i] * f;
+        }
+        m = mn;
+    };
+    some(0);                                                    // apart: nothing to rescale
+    for (int i0 = AT_ONCE; __any(i0 < nsp); i0 += AT_ONCE) some(i0);
     if (nsp == 0) return;
     const float inv = tot == 0.f ? 0.f : a.v_scale / tot;
     *(u32x2_t*)(a.out + (size_t)token * a.ldo_b + (size_t)head * 256 + l * 8) =
@@ -1031,12 +1040,16 @@ Plan make_plan(int T, int B, int max_kv, int n_q, int n_kv, int cus) {
     const long long bound = (long long)T * g / p.R + B;         // tiles per key/value head, at most
     const long long some = tiles(p.R);
     const long long slots = p.R == 256 ? cus : two;
-    // no range under eight steps of a workgroup, 1024 or 512 keys (us at half / at it / at twice: 32 single tokens x 2000 keys 53.9 / 50.6 /
-    // 50.9, 4 x 20000 65.5 / 64.8 / 83.8; 8 blocks of 128 tokens x 2000 49.8 / 48.5 / 57.3, 8 of 200 x 4000 108 / 101 / 102), and no more
-    // partial outputs than 64 MiB
-    const int least = p.R <= 32 ? 1024 : 512;
+    // The shortest range.  Tiles on less than a quarter of the chip wait for latency, and the chain of a range's tiles is what they wait
+    // for: 128 keys, once there are enough of them to pay for the second kernel (us uncut / cut into 128 ..: one token on 8 heads, 700 keys
+    // 13.2 / 14.1, 1000 15.6 / 14.4, 1500 19.8 / 14.4, 5000 50 / 15.7; a block of 32 700 17.5 / 16.4, 1500 26 / 17.2; 100 tokens 500 21.2 / 18.5,
+    // 1500 42.5 / 20.2).  Otherwise eight steps of a workgroup, 1024 or 512 keys (us at half / at it / at twice: 32 single tokens x 2000 keys
+    // 53.9 / 50.6 / 50.9, 8 blocks of 128 tokens x 2000 49.8 / 48.5 / 57.3, 8 of 200 x 4000 108 / 101 / 102).  No more partial outputs than
+    // 64 MiB.
+    const bool idle = some * n_kv * 4 < slots;
+    const int least = idle ? 128 : p.R <= 32 ? 1024 : 512;
     const long long row_bytes = (long long)T * n_q * (HEAD_DIM + 2) * 4;
-    long long most = max_kv / least;
+    long long most = idle && max_kv < (p.R <= 32 ? 768 : 512) ? 1 : max_kv / least;
     if (most > (64LL << 20) / row_bytes) most = (64LL << 20) / row_bytes;
     if (most > 256) most = 256;
     // few tiles: one round of equal units.  Many: about four rounds, so that sequences of unequal length even out
@@ -1125,7 +1138,7 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     const long long rows = (long long)T * n_q;
     auto join = [&](auto tile_rows) {
         constexpr int R = decltype(tile_rows)::value;
-        if (p.max_ranges <= FEW_RANGES) hipLaunchKernelGGL(paged_attn_join_few_kernel<R>, dim3((unsigned)(((long long)T * ((n_q + 1) / 2) + 3) / 4)), dim3(256), 0, st, a);
+        if (p.max_ranges <= AT_ONCE || rows > 4LL * coda_device_cus()) hipLaunchKernelGGL(paged_attn_join_rows_kernel<R>, dim3((unsigned)(((long long)T * ((n_q + 1) / 2) + 3) / 4)), dim3(256), 0, st, a);
         else hipLaunchKernelGGL(paged_attn_join_kernel<R>, dim3((unsigned)rows), dim3(256), 0, st, a);
     };
     if (p.R == 16) join(std::integral_constant<int, 16>{});

@@ -163,9 +163,10 @@ def test_attention_head_groups(g, n, cache):
 
 @pytest.mark.parametrize("cache", ["bf16", "e4m3"])
 @pytest.mark.parametrize("lens,past", [([1], [5000]), ([1, 1, 1], [3000, 10, 1700]), ([20, 1], [2500, 900]), ([60, 2], [4000, 4]),
-                                       ([200], [2000])])
+                                       ([200], [2000]), ([300], [4000]), ([20] * 13, [2000 - 150 * i for i in range(13)])])
 def test_attention_ranges_of_keys(lens, past, cache):
-    """Few rows over many keys: the keys are cut into ranges and joined; short sequences of the batch have one range."""
+    """Few rows over many keys: the keys are cut into ranges and joined; short sequences of the batch have one range.  The last two: more
+    rows and ranges than are joined in one step."""
     b = Batch(lens, past, 32, 4, 2, cache, seed=5)
     assert _lib.load().coda_paged_attn_workspace_bytes(b.T, b.B, max(b.total), 4, 2) > 0
     for mask in (0, 1):

@@ -86,9 +86,9 @@ def test_attn_workspace_sizes():
     assert size(1, 1, 4096, 16, 8) > 0
     assert size(0, 1, 4096, 16, 8) == 0 and size(1, 1, 4096, 16, 7) == 0      # sizes that the call itself refuses
     for T, B, kv in ((1, 1, 40960), (4, 4, 40960), (128, 128, 2048), (1024, 32, 384), (8192, 8, 4096)):
-        # a head, and a partial output and two numbers per range, token and head; no ranges under 512 keys, nor over 64 MiB of them
+        # a head, and a partial output and two numbers per range, token and head; no ranges under 128 keys, nor over 64 MiB of them
         n = size(T, B, kv, 16, 8)
-        assert n == 0 or (n - 256) % (T * 16 * 130 * 4) == 0 and n - 256 <= min(kv // 512 * T * 16 * 130 * 4, 64 << 20)
+        assert n == 0 or (n - 256) % (T * 16 * 130 * 4) == 0 and n - 256 <= min(kv // 128 * T * 16 * 130 * 4, 64 << 20)
 
 
 LORA = dict(X=P, ldx=256, A=P, Bw=P, scale=None, seq_start=P, adapter=P, B=2, T=4, n_adapters=3, rank=64, R=P, ldr=512, C=P, ldc=512, N=512,
