@@ -636,11 +636,15 @@ __global__ __launch_bounds__(256, RG == 1 && F8 ? 3 : 2) void paged_attn_few_ker
 // Many rows: NW waves of 32 rows each share a double-buffered stream of 64-key tiles, one barrier a tile.
 //
 // What bounds it: the chain products - maximum - exponentials - products of a wave, which the other wave of its SIMD only partly
-// covers, and the LDS reads of every fragment for only 32 rows.  Measured, 16 heads on 8: 8 x 2048 tokens, no mask 312 us = 880 TFLOP/s,
-// causal 184 us; 2 x 8192 no mask 1109 us = 991 TFLOP/s, of the 1257 that a large matrix product reaches on this card.  Whole bf16 tiles
-// straight to LDS instead of through registers: 8 x 2048 causal 184 / 191 us (one card, in turn), 8 x 200 behind 4000 keys 106 / 117, 16 x
-// 64 behind 2000 54.5 / 57.  Slower or no faster, against 303 .. 314 us for 8 x 2048 without mask through registers: the two halves of the
-// workgroup one barrier apart (341), the softmax of a tile beside the scores of the next (311), wave priorities around the products (316).
+// covers, and the LDS reads of every fragment for only 32 rows.  The weights are a bf16 pair, so of three matrix instructions two are the
+// second product's.  Measured, 16 heads on 8: 8 x 2048 tokens, no mask 386 us = 712 TFLOP/s (with the remainders, which are not counted,
+// the matrix unit does half as much again), causal 225 us; 2 x 8192 no mask 1419 us = 775 TFLOP/s; a large matrix product reaches 1257 on
+// this card.  One bf16 weight in place of the pair took 291, 175 and 1025 us, with an error of 0.0022 of the result where its own rounding
+// to bf16 is 0.0017: a call's rows would be less exact for being many.
+// With one weight a key were measured: whole bf16 tiles straight to LDS instead of through registers: 8 x 2048 causal 184 / 191 us (one
+// card, in turn), 8 x 200 behind 4000 keys 106 / 117, 16 x 64 behind 2000 54.5 / 57.  Slower or no faster, against 303 .. 314 us for 8 x
+// 2048 without mask through registers: the two halves of the workgroup one barrier apart (341), the softmax of a tile beside the scores of
+// the next (311), wave priorities around the products (316).
 constexpr int MANY_TILE = 64;
 constexpr int MANY_BUF = 2 * MANY_TILE * 256;                   // K and V image: 32 KiB
 
@@ -807,14 +811,23 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
                 psum += p;
             }
         l_run += psum;
-        // weights rounded to bf16 for the matrix unit (half a step: 2^-8 of each weight at most); the sum l keeps them in fp32
+        // the weights as a bf16 pair, as in the `few` kernel: each V fragment that was read from LDS enters two products
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
-            bf16x8_t pf;
+            bf16x8_t ph, pl;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[st >> 1][8 * (st & 1) + j];
+            for (int j = 0; j < 8; ++j) {
+                const float p = s[st >> 1][8 * (st & 1) + j];
+                ph[j] = (__bf16)p;
+                pl[j] = (__bf16)(p - (float)ph[j]);
+            }
+            bf16x8_t vf[4];
 #pragma unroll
-            for (int db = 0; db < 4; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rd.v(vimg, st, db), pf, o[db], 0, 0, 0);
+            for (int db = 0; db < 4; ++db) vf[db] = rd.v(vimg, st, db);
+#pragma unroll
+            for (int db = 0; db < 4; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db], pl, o[db], 0, 0, 0);
+#pragma unroll
+            for (int db = 0; db < 4; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db], ph, o[db], 0, 0, 0);
         }
     };
 
@@ -1037,11 +1050,11 @@ Plan make_plan(int T, int B, int max_kv, int n_q, int n_kv, bool slanted, int cu
     };
     const long long two = 2LL * cus;                            // workgroups of 256 threads that are resident at once
     // us with tiles of so many rows, 16 heads on 8, bf16:
-    //   16 / 32      32 sequences x 2000 keys: rho 8 51 / 53, rho 16 51 / 53, rho 24 57 / 53
-    //   32 / 128     32 x 1000: rho 48 37 / 41, rho 64 40 / 45, rho 80 59 / 47; 128 x 1500: 183 / 216, 185 / 167, 246 / 176; 8 x 4000:
-    //                48 / 42, 49 / 44, 62 / 45; all tiles resident and keys short, 8 x 300: rho 64 13.7 / 16.7, rho 128 14.5 / 17.7
-    //   128 / 256    16 x 2000: rho 256 73 / 84; 4 x 1000: rho 768 50 / 48, rho 1024 55 / 63; 8 x 2048 new: 327 / 306, 2 x 8192 new 1209 /
-    //                1115, behind 8000 keys 1 x 1000 123 / 110, but 1 x 2048 new 72 / 79 (too few tiles for the chip)
+    //   16 / 32      32 sequences x 2000 keys: rho 8 51 / 53, rho 16 51 / 53, rho 24 58 / 53
+    //   32 / 128     32 x 1000: rho 48 38 / 44, rho 64 41 / 50, rho 80 58 / 53; 128 x 1500: 182 / 224, 183 / 190, 246 / 200; 8 x 4000:
+    //                43 / 45, 50 / 47, 62 / 49; all tiles resident and keys short, 8 x 300: rho 64 14.1 / 20.1, rho 128 14.9 / 21.0
+    //   128 / 256    16 x 2000: rho 256 84 / 102; 4 x 1000: rho 768 52.6 / 50.7, rho 1024 57.6 / 56.9; 8 x 2048 new: 403 / 402, 2 x 8192
+    //                new 1547 / 1522, behind 8000 keys 1 x 1000 128 / 123, but 2 x 2048 new 74 / 88 (too few tiles for the chip)
     // (64 rows on eight waves lost to 32 or 128 everywhere.)
     if (rho <= 16) p.R = 16;
     else if (rho <= 64 || (rho <= 128 && max_kv < 2048 && tiles(32) * n_kv <= two)) p.R = 32;

@@ -275,8 +275,8 @@ int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out, long long 
  * does not see have no influence on it, whatever their slots hold; a NaN score or an infinity or NaN in V that it does see makes
  * its output (of the feature, for V) non-finite.
  * max_kv: host-side bound of kv_len, at most max_pages * page_size and 2^30 (keys from max_kv on are not seen): it sizes the launch.
- * Scores, maxima, sums and outputs are fp32; weights enter the second product as bf16 (a bf16 pair where there are at most 64
- * rows per sequence and key/value head).  T * n_q / n_kv is at most 2^28.  scale > 0, and scale * 1.4427 (e4m3: * k_scale) within [1e-30, 1e30].
+ * Scores, maxima, sums and outputs are fp32; weights enter the second product as a bf16 pair (value and remainder: 16 significant
+ * bits).  T * n_q / n_kv is at most 2^28.  scale > 0, and scale * 1.4427 (e4m3: * k_scale) within [1e-30, 1e30].
  * workspace: coda_paged_attn_workspace_bytes(T, B, max_kv, n_q, n_kv) bytes (may be 0), 16-byte aligned, contents irrelevant before
  * and after; calls that may run at the same time need one each. */
 long long coda_paged_attn_workspace_bytes(int T, int B, int max_kv, int n_q, int n_kv);

@@ -566,3 +566,38 @@ def test_attention_tile_order(B, mask):
     b.pos0[0] = 10 ** 6                                      # far behind every key: all rows see all of them
     b.kv_len[2 % B] = 0
     check(attn(b, mask), b, mask=mask)
+
+
+# ------------------------------------------------------------------------------------------------ how exact the weights are
+def check_pair(out, b, **kw):
+    """check() for weights that keep 16 bits: |out - ref| <= 2^-8 |ref| (the bf16 result) + 2 (2^-16 + ds + sums) sum p |v|.  A weight is
+    a bf16 value and the bf16 value of its remainder: half a step of half a step, 2^-8 * 2^-8.  ds: a score is a sum of 128 products
+    in fp32.  sums: two products a key, added up in fp32, and 2^-20 for the device's exp2.  Numerator and denominator, hence 2."""
+    ref, mag, ds = attn_ref(b, **kw)
+    n = b.starts[-1]
+    got = out[:n, :b.n_q * D].to(F64).cpu()
+    sums = 2 * max(b.total) * 2.0 ** -24 + 2.0 ** -20
+    tol = 2.0 ** -8 * ref[:n].abs() + 2 * (2.0 ** -16 + 128 * 2.0 ** -24 * ds[:n] + sums) * mag[:n] * (1 + 2.0 ** -8) + 1e-30
+    err = (got - ref[:n]).abs()
+    bad = err > tol
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} outputs, worst {(err / tol).max()} of the bound, rows {bad.any(1).nonzero()[:4, 0].tolist()} .."
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("page", [16, 10])
+@pytest.mark.parametrize("lens,past,n_q,n_kv", [
+    ([1, 1, 1], [40, 3, 17], 16, 8),                         # tiles of 16 rows
+    ([16, 9], [24, 31], 6, 2),                               # of 32
+    ([66, 60], [3, 10], 4, 2),                               # of 32, more than 64 rows a sequence
+    ([100, 90], [10, 0], 4, 2),                              # of 128
+    ([90], [430], 4, 2),                                     # of 128, keys in ranges
+    ([300, 1, 1, 1], [0, 50, 7, 31], 16, 8),                 # of 128: single tokens beside a prompt
+    ([200], [0], 320, 40),                                   # of 256
+    ([1] * 9 + [120], [20 + i for i in range(9)] + [0], 16, 8),     # of 32: a prompt among single tokens
+])
+def test_attention_weights_keep_sixteen_bits(lens, past, n_q, n_kv, page, cache):
+    """Whatever tiles a call is cut into and whatever else is in it.  Small queries: weights of like size, whose roundings would show."""
+    b = Batch(lens, past, page, n_q, n_kv, cache, seed=81)
+    b.q *= 0.4
+    for mask in (0, 1):
+        check_pair(attn(b, mask), b, mask=mask)
