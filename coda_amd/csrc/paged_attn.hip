@@ -522,8 +522,9 @@ __global__ __launch_bounds__(256, RG == 1 && F8 ? 3 : 2) void paged_attn_few_ker
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
             if (__any(mx > m_run[rg] + RESCALE_THR)) {
-                const float m_new = fmaxf(m_run[rg], mx);
-                // a row that has seen no key yet keeps -inf and nothing to scale
+                // only rows that ask for it, so that no row's bits depend on what another one sees; one that has seen no key yet keeps -inf
+                // and nothing to scale
+                const float m_new = mx > m_run[rg] + RESCALE_THR ? mx : m_run[rg];
                 const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[rg] - m_new);
                 l_run[rg] *= alpha;
                 m_run[rg] = m_new;
@@ -791,7 +792,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void paged_attn_many_kern
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[k2][i]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
         if (__any(mx > m_run + RESCALE_THR)) {
-            const float m_new = fmaxf(m_run, mx);
+            const float m_new = mx > m_run + RESCALE_THR ? mx : m_run;      // only rows that ask for it, as above
             const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
             l_run *= alpha;
             m_run = m_new;

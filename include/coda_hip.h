@@ -273,7 +273,8 @@ int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out, long long 
  * (the denoiser's attention).  mask_block m > 0: token i sees the keys before the end of its block of m positions,
  * j < ((pos0[b] + i) / m + 1) * m (1: causal).  A token that sees no key, or only scores of -infinity, gets zeros.  Keys a token
  * does not see have no influence on it, whatever their slots hold; a NaN score or an infinity or NaN in V that it does see makes
- * its output (of the feature, for V) non-finite.
+ * its output (of the feature, for V) non-finite.  The same call has the same bits every time; how the keys are cut and in which
+ * order parts are added follows from the sizes and all sequences' lengths, so a request's last bits may differ in another batch.
  * max_kv: host-side bound of kv_len, at most max_pages * page_size and 2^30 (keys from max_kv on are not seen): it sizes the launch.
  * Scores, maxima, sums and outputs are fp32; weights enter the second product as a bf16 pair (value and remainder: 16 significant
  * bits).  T * n_q / n_kv is at most 2^28.  scale > 0, and scale * 1.4427 (e4m3: * k_scale) within [1e-30, 1e30].

@@ -601,3 +601,19 @@ def test_attention_weights_keep_sixteen_bits(lens, past, n_q, n_kv, page, cache)
     b.q *= 0.4
     for mask in (0, 1):
         check_pair(attn(b, mask), b, mask=mask)
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3])
+@pytest.mark.parametrize("lens,past", [([7], [60]), ([16, 2], [90, 10]), ([60, 3], [100, 20]), ([140], [77]), ([300, 9], [40, 600])])
+def test_attention_unseen_keys_move_no_bit(lens, past, seed):
+    """A key that only the last token of a sequence sees, with a score far above all others: every other row keeps its bits, also those
+    that share a wave with it and its rescaling."""
+    b = Batch(lens, past, 16, 4, 2, seed=90 + seed)
+    clean = attn(b, 1).clone()
+    last, row = b.total[0] - 1, b.starts[1] - 1
+    q = b.q[row, :b.n_q * D].view(b.n_kv, b.n_q // b.n_kv, D)[:, 0]
+    b.pages(b.k)[int(b.table[0, last // b.page]), :, last % b.page] = 8 * q         # a score of 8 |q|^2 / sqrt(128), about 200
+    out = attn(b, 1)
+    others = torch.tensor([r for r in range(b.starts[-1]) if r != row])
+    assert not torch.equal(out[row], clean[row])
+    assert torch.equal(out[others], clean[others])
