@@ -52,6 +52,15 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs& a, int slot) {
     return {q.s0 + k * TM, min(q.n - k * TM, TM), (unsigned)q.x < (unsigned)a.n_adapters ? q.x : -1, 0};
 }
 
+// x as a bf16 value and its bf16 remainder.  bf16 rounds to infinity a little before fp32 ends: such an x is bf16's largest value and the
+// rest; an infinity has no remainder (inf - inf would make it a NaN).
+__device__ __forceinline__ void bf16_pair(float x, __bf16& h, __bf16& l) {
+    float f = round_bf16(x);
+    if (fabsf(f) == INFINITY && fabsf(x) != INFINITY) f = copysignf(0x1.fep127f, x);
+    h = (__bf16)f;
+    l = (__bf16)(fabsf(f) == INFINITY ? 0.f : x - f);
+}
+
 // U of 16 MT tokens, 16 RT ranks (those beyond the adapter's are computed from its last row and dropped).
 // Steps of 256 elements: rows of X and A come in as contiguous 512 bytes through registers (those of the next two steps fly under this
 // one's products: 7.7 us, one step ahead 8.4, 32 blocks of 32 tokens, rank 64, K 6144) into an LDS image, 16-byte chunk ch of row r at ch ^ (r & 15), and the four waves take 64 elements of each step.
@@ -215,9 +224,10 @@ __global__ __launch_bounds__(256, 2) void lora_up_kernel(LoraArgs a) {
         bf16x4_t h4, l4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float x = s * v[j];
-            h4[j] = (__bf16)x;
-            l4[j] = (__bf16)(x - (float)h4[j]);
+            __bf16 h, l;
+            bf16_pair(s * v[j], h, l);
+            h4[j] = h;
+            l4[j] = l;
         }
         *(bf16x4_t*)&us[0][m][r0] = h4;
         *(bf16x4_t*)&us[1][m][r0] = l4;
@@ -341,9 +351,10 @@ __global__ __launch_bounds__(1024) void lora_one_kernel(LoraArgs a) {
             bf16x4_t h4, l4;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float x = s * v[j];
-                h4[j] = (__bf16)x;
-                l4[j] = (__bf16)(x - (float)h4[j]);
+                __bf16 h, l;
+                bf16_pair(s * v[j], h, l);
+                h4[j] = h;
+                l4[j] = l;
             }
             *(bf16x4_t*)&us[0][col][16 * wave + 4 * quad] = h4;
             *(bf16x4_t*)&us[1][col][16 * wave + 4 * quad] = l4;

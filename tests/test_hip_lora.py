@@ -163,3 +163,23 @@ def test_lora_starts_that_make_no_sense(starts, rank):
     c.call(out=guard[32:32 + c.T])
     torch.cuda.synchronize()
     assert (guard[:32] == 7).all() and (guard[32 + c.T:] == 7).all()
+
+
+@pytest.mark.parametrize("rank", [16, 24, 64])
+def test_lora_infinities_and_the_end_of_the_range(rank):
+    """An infinity in X comes out as the infinity that the formula gives, not as a NaN; products X A^T between bf16's largest value and fp32's
+    are kept.  One launch (ranks 16, 24) and two."""
+    c = Case([3, 4, 2], [0, 1, -1], 256, 264, rank, n=2, scale=False)
+    assert (_lib.load().coda_lora_workspace_bytes(c.T, c.B, c.N, c.K, rank) == 0) == (rank < 64)
+    c.a[0], c.b[0] = c.a[0].abs() + 2.0 ** -6, c.b[0].abs() + 2.0 ** -6       # no zeros: 0 * inf would be a NaN by right
+    c.x[0, 5], c.x[1, 9] = float("inf"), float("-inf")
+    c.a[1], c.b[1] = 0, 0
+    c.a[1, 3, :2], c.b[1, :, 3] = 1, 2.0 ** -10                # U[3] = x0 + x1, all else 0
+    c.x[3, :2] = torch.tensor([3.3895313892515355e38, 1e36])   # bf16's largest value, and beyond half a step of it
+    c.x[4, :2] = -c.x[3, :2]
+    out = c.call()
+    torch.cuda.synchronize()
+    assert (out[0, :c.N] == float("inf")).all() and (out[1, :c.N] == float("-inf")).all()
+    out[0, :c.N], out[1, :c.N] = c.r[0, :c.N].to(DEV), c.r[1, :c.N].to(DEV)
+    c.x[0], c.x[1] = 0, 0
+    c.check(out)
