@@ -418,7 +418,7 @@ long long plan_bytes(const Plan& p, int T, int rank) { return p.one ? 0 : p.nslo
 }  // namespace
 
 extern "C" long long coda_lora_workspace_bytes(int T, int B, int N, int K, int rank) {
-    if (T <= 0 || B <= 0 || N <= 0 || K <= 0 || rank <= 0) return 0;
+    if (T <= 0 || B <= 0 || N <= 0 || K <= 0 || rank <= 0 || T > 1 << 28 || N > 1 << 30 || K > 1 << 30 || rank > 128) return 0;
     return plan_bytes(make_plan(T, B, N, K, rank, coda_device_cus()), T, rank);
 }
 
@@ -429,6 +429,7 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
     if (B <= 0 || T <= 0 || n_adapters <= 0 || N <= 0 || K <= 0) return coda_refuse(who, CODA_ERR_SHAPE, "a size is not positive");
     // running sums over 64 sequences of tiles stay below 2^31 even for starts that make every sequence T rows long
     if (T > 1 << 28) return coda_refuse(who, CODA_ERR_SHAPE, "T exceeds 2^28");
+    if (N > 1 << 30 || K > 1 << 30) return coda_refuse(who, CODA_ERR_SHAPE, "N or K exceeds 2^30");       // sums with tile sizes would wrap
     if (rank <= 0 || rank % 8 || rank > 128) return coda_refuse(who, CODA_ERR_SHAPE, "rank is a multiple of 8 up to 128");
     if (K % 64 || N % 8) return coda_refuse(who, CODA_ERR_SHAPE, "K % 64 or N % 8");
     if (ldx < K || ldr < N || ldc < N) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");

@@ -31,6 +31,7 @@ int coda_check_pages(const char* who, const void* k_cache, const void* v_cache, 
     if (cache_type == CODA_CACHE_E4M3 && (!(k_scale > 0.f) || !(v_scale > 0.f) || k_scale > 1e30f || v_scale > 1e30f || k_scale < 1e-30f || v_scale < 1e-30f))
         return coda_refuse(who, CODA_ERR_ARG, "scales of an e4m3 cache lie in [1e-30, 1e30]");
     if (max_pages <= 0 || num_pages <= 0 || page_size <= 0 || ld_table < max_pages) return coda_refuse(who, CODA_ERR_SHAPE, "page table or page size");
+    if (n_kv > MAX_HEADS) return coda_refuse(who, CODA_ERR_SHAPE, "too many heads");        // the size of a page would wrap
     if ((long long)max_pages * page_size > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "max_pages * page_size exceeds 2^31 - 1");
     const int elt = cache_type == CODA_CACHE_E4M3 ? 1 : 2;
     if (page_stride < (long long)n_kv * page_size * HEAD_DIM) return coda_refuse(who, CODA_ERR_SHAPE, "page_stride is smaller than a page");
@@ -200,7 +201,7 @@ extern "C" int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out,
                                  float v_scale, int n_q, int n_kv, float eps, int flags, void* stream) {
     const char* who = "coda_paged_append";
     if (B <= 0 || T <= 0 || n_q <= 0 || n_kv <= 0 || max_pos <= 0) return coda_refuse(who, CODA_ERR_SHAPE, "a size is not positive");
-    if ((long long)n_q + 2LL * n_kv > (1 << 20)) return coda_refuse(who, CODA_ERR_SHAPE, "too many heads");
+    if ((long long)n_q + 2LL * n_kv > MAX_HEADS) return coda_refuse(who, CODA_ERR_SHAPE, "too many heads");
     if (ld_qkv < ((long long)n_q + 2LL * n_kv) * HEAD_DIM || ld_q < (long long)n_q * HEAD_DIM) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");
     if (!qkv || !q_out || !cos || !sin || !seq_start || !pos0) return coda_refuse(who, CODA_ERR_ARG, "null pointer");
     if (!q_weight != !k_weight) return coda_refuse(who, CODA_ERR_ARG, "q_weight and k_weight come together or not at all");

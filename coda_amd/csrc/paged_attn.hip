@@ -1095,6 +1095,7 @@ long long plan_bytes(const Plan& p, int T, int n_q) {
 
 extern "C" long long coda_paged_attn_workspace_bytes(int T, int B, int max_kv, int n_q, int n_kv) {
     if (T <= 0 || B <= 0 || max_kv < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv) return 0;
+    if ((long long)T * n_q > 0x7fffffffLL) return 0;            // the call refuses these too
     return plan_bytes(make_plan(T, B, max_kv, n_q, n_kv, false, coda_device_cus()), T, n_q);
 }
 

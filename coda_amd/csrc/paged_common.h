@@ -7,6 +7,7 @@
 namespace paged {
 
 constexpr int HEAD_DIM = 128;
+constexpr int MAX_HEADS = 1 << 20;
 
 // n / d for 0 <= n < 2^31 and 1 <= d < 2^31 as multiply-high, add, shift (round-up method: magic = ceil(2^(32+s) / d) - 2^32
 // with s = ceil(log2 d); the sum of the high product and n stays below 2^32).  Page sizes are the caller's and need not be

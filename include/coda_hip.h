@@ -267,7 +267,7 @@ int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out, long long 
                       void* v_cache, long long page_stride, int num_pages, int page_size, int cache_type, float k_scale,
                       float v_scale, int n_q, int n_kv, float eps, int flags, void* stream);
 
-/* Attention of the new tokens' queries over the cache: out_i = softmax_j(scale q_i . K_j) V, n_q % n_kv == 0, from one token a
+/* Attention of the new tokens' queries over the cache: out_i = softmax_j(scale q_i . K_j) V, n_q % n_kv == 0, n_kv at most 2^20, from one token a
  * sequence (decode) to whole prompts.  q and out bf16 [T, n_q * 128] (out apart from q and the cache).  Sequence b has
  * kv_len[b] keys, positions 0 .. kv_len[b]-1 (int32 [B]).  mask_block 0: a token sees all of them, later positions included
  * (the denoiser's attention).  mask_block m > 0: token i sees the keys before the end of its block of m positions,
@@ -292,7 +292,7 @@ int coda_paged_attn(const void* q, long long ld_q, void* out, long long ld_out, 
  * X bf16 [T, K] (the projection's input), R bf16 [T, N] (its output, e.g. of coda_gemm_bf16 CODA_EPI_PLAIN), C bf16 [T, N]: R
  * itself (in place) or memory apart from R and X.  A bf16 [n_adapters, rank, K], B bf16 [n_adapters, N, rank], both dense; scale
  * fp32 [n_adapters] on the device or NULL (1); adapter int32 [B], a value outside [0, n_adapters) means none: C[t] = R[t].
- * rank is a multiple of 8 up to 128 (adapters of smaller rank: zero rows of A), K % 64 == 0, N % 8 == 0, T at most 2^28.  Both products are summed in
+ * rank is a multiple of 8 up to 128 (adapters of smaller rank: zero rows of A), K % 64 == 0, N % 8 == 0, T at most 2^28, N and K at most 2^30.  Both products are summed in
  * fp32 and the result is rounded once; X A^T enters the second one as a bf16 pair (16 significant bits).
  * workspace: coda_lora_workspace_bytes(T, B, N, K, rank) bytes, 16-byte aligned, contents irrelevant before and after; calls
  * that may run at the same time need one each. */

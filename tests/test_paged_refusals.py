@@ -91,6 +91,24 @@ def test_attn_workspace_sizes():
         assert n == 0 or (n - 256) % (T * 16 * 130 * 4) == 0 and n - 256 <= min(kv // 128 * T * 16 * 130 * 4, 64 << 20)
 
 
+@pytest.mark.parametrize("name,change,code,words", [
+    # n_kv * page_size * 128 is 2^64: a page_stride of any length would pass for a page
+    ("coda_paged_attn", dict(T=1, n_q=1 << 30, n_kv=1 << 30, ld_q=1 << 38, ld_out=1 << 38, page_size=1 << 27, page_stride=2048), "SHAPE", "heads"),
+    ("coda_paged_attn", dict(T=1, n_q=(1 << 20) + 1, n_kv=(1 << 20) + 1, ld_q=1 << 38, ld_out=1 << 38, page_stride=1 << 40), "SHAPE", "heads"),
+    ("coda_lora_bf16", dict(N=2147483640, ldr=1 << 31, ldc=1 << 31), "SHAPE", "2^30"),
+    ("coda_lora_bf16", dict(K=2147483584, ldx=1 << 31), "SHAPE", "2^30"),
+])
+def test_sizes_whose_sums_would_wrap(name, change, code, words):
+    refused(name, {"coda_paged_attn": ATTN, "coda_lora_bf16": LORA}[name], change, code, words)
+
+
+def test_workspaces_of_sizes_that_would_wrap():
+    lib, big = _lib.load(), (1 << 31) - 1
+    assert lib.coda_paged_attn_workspace_bytes(big, big, big, big, 1) == 0 and lib.coda_paged_attn_workspace_bytes(1 << 30, 1, 1 << 30, 8, 8) == 0
+    assert lib.coda_lora_workspace_bytes(4, 2, big, 64, 8) == 0 and lib.coda_lora_workspace_bytes(4, 2, 64, big, 8) == 0
+    assert lib.coda_lora_workspace_bytes(big, 2, 64, 64, 8) == 0 and lib.coda_lora_workspace_bytes(4, 2, 64, 64, big) == 0
+
+
 LORA = dict(X=P, ldx=256, A=P, Bw=P, scale=None, seq_start=P, adapter=P, B=2, T=4, n_adapters=3, rank=64, R=P, ldr=512, C=P, ldc=512, N=512,
             K=256, workspace=P, workspace_bytes=1 << 30, stream=None)
 
