@@ -441,7 +441,7 @@ extern "C" int coda_lora_bf16(const void* X, long long ldx, const void* A, const
         return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_lora_workspace_bytes");
     if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
     const long long downs = rank > 64 ? (p.nslots * p.ksplit + 7) / 8 * 16 : p.nslots * p.ksplit, ups = p.nslots * ((N + p.nslice - 1) / p.nslice);
-    if (downs > 0x7fffffffLL || ups > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
+    if (!p.one && (!grid_fits(downs, 256) || !grid_fits(ups, 256))) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
     LoraArgs a;
     a.x = (const char*)X; a.ldx_b = ldx * 2;
     a.a = (const char*)A; a.b = (const char*)Bw; a.scale = scale;

@@ -231,7 +231,7 @@ extern "C" int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out,
     a.parts = (n_heads + 15) / 16;
     while (a.parts * 4 < n_heads && (long long)T * a.parts * 2 <= fill) a.parts *= 2;
     const long long wgs = ((long long)T * a.parts + 3) / 4;
-    if (wgs > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many rows for one launch");
+    if (!grid_fits(wgs, 256)) return coda_refuse(who, CODA_ERR_SHAPE, "too many rows for one launch");
     const dim3 grid((unsigned)wgs), block(256);
     hipStream_t st = (hipStream_t)stream;
     if (f8 && stepwise) hipLaunchKernelGGL((paged_append_kernel<true, true>), grid, block, 0, st, a);

@@ -1131,7 +1131,7 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     const long long need = plan_bytes(p, T, n_q);
     if (need > 0 && (!workspace || workspace_bytes < need)) return coda_refuse(who, CODA_ERR_ARG, "workspace is smaller than coda_paged_attn_workspace_bytes");
     if ((uintptr_t)workspace & 15) return coda_refuse(who, CODA_ERR_ALIGN, "the workspace starts on 16 bytes");
-    if (p.wgs > 0x7fffffffLL) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
+    if (!grid_fits(p.wgs, p.R == 256 ? 512 : 256)) return coda_refuse(who, CODA_ERR_SHAPE, "too many tiles for one launch");
     a.q = (const char*)q; a.ldq_b = ld_q * 2;
     a.out = (char*)out; a.ldo_b = ld_out * 2;
     a.seq_start = seq_start; a.pos0 = pos0; a.kv_len = kv_len;

@@ -151,6 +151,9 @@ __device__ __forceinline__ Seq seq_of_item(const SeqArrays& a, SeqBlock& blk, in
     return {-1, 0, 0, 0, 0};
 }
 
+// A launch holds fewer than 2^32 work items: what has more is refused in words before anything is launched.
+inline bool grid_fits(long long workgroups, int threads) { return workgroups * threads <= 0xffffffffLL; }
+
 }  // namespace paged
 
 // Host-side checks common to the entry points that take a paged cache; 0 or an error code (with words).

@@ -113,6 +113,17 @@ LORA = dict(X=P, ldx=256, A=P, Bw=P, scale=None, seq_start=P, adapter=P, B=2, T=
             K=256, workspace=P, workspace_bytes=1 << 30, stream=None)
 
 
+@pytest.mark.parametrize("name,change,words", [
+    ("coda_paged_append", dict(T=(1 << 26) + 1, n_q=1, n_kv=1), "too many rows"),                    # four tokens a workgroup of 256
+    ("coda_paged_attn", dict(T=1 << 24, B=1 << 24, n_q=1, n_kv=1), "too many tiles"),                # 2^24 sequences of a token
+    ("coda_paged_attn", dict(T=3200, B=1 << 22, n_q=8), "too many tiles"),                            # almost all sequences empty
+    ("coda_lora_bf16", dict(T=1 << 24, B=1 << 24, workspace_bytes=1 << 40), "too many tiles"),
+])
+def test_launches_of_too_many_work_items(name, change, words):
+    """2^32 work items and more are no launch; fewer than 2^31 workgroups all the same."""
+    refused(name, {"coda_paged_append": APPEND, "coda_paged_attn": ATTN, "coda_lora_bf16": LORA}[name], change, "SHAPE", words)
+
+
 @pytest.mark.parametrize("change,code,words", [
     (dict(B=0), "SHAPE", "positive"), (dict(T=0), "SHAPE", "positive"), (dict(T=-3), "SHAPE", "positive"), (dict(n_adapters=0), "SHAPE", "positive"),
     (dict(T=(1 << 28) + 1), "SHAPE", "2^28"), (dict(N=0), "SHAPE", "positive"), (dict(K=0), "SHAPE", "positive"), (dict(rank=0), "SHAPE", "rank"), (dict(rank=12), "SHAPE", "rank"),
