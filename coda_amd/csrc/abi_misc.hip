@@ -40,7 +40,11 @@ int coda_device_cus() {
 
 int coda_ensure_dyn_lds(const void* func, int bytes) {
     int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess) return CODA_ERR_LAUNCH;
+    const hipError_t d = hipGetDevice(&dev);
+    if (d != hipSuccess) {
+        coda_set_last_error("hipGetDevice", d);
+        return CODA_ERR_LAUNCH;
+    }
     if (dev >= 0 && dev < MAX_DEV) {
         std::lock_guard<std::mutex> lk(g_mu);
         for (auto& e : g_dev[dev].lds)

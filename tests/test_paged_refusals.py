@@ -3,6 +3,7 @@ words before anything is launched, so none of this needs a GPU - and none of the
 import os
 
 import pytest
+import torch
 
 from coda_amd import _lib
 
@@ -78,6 +79,14 @@ def test_append_refuses(change, code, words):
 ])
 def test_attn_refuses(change, code, words):
     refused("coda_paged_attn", ATTN, change, code, words)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what a machine without a GPU answers")
+def test_no_device_is_said_and_not_an_older_error():
+    refused("coda_paged_append", APPEND, dict(flags=2), "ARG", "flag")
+    with pytest.raises(_lib.CodaHipError) as e:
+        _lib.call("coda_paged_attn", *ATTN.values())
+    assert "CODA_ERR_LAUNCH hipGetDevice: " in str(e.value), str(e.value)
 
 
 def test_attn_workspace_sizes():
