@@ -617,3 +617,38 @@ def test_attention_unseen_keys_move_no_bit(lens, past, seed):
     others = torch.tensor([r for r in range(b.starts[-1]) if r != row])
     assert not torch.equal(out[row], clean[row])
     assert torch.equal(out[others], clean[others])
+
+
+def uncut(b):
+    """No ranges of keys: no workspace."""
+    return _lib.load().coda_paged_attn_workspace_bytes(b.T, b.B, max(b.total), b.n_q, b.n_kv) == 0
+
+
+@pytest.mark.parametrize("mask", [1, 64])
+@pytest.mark.parametrize("B,n_q,n_kv", [(1, 2, 1), (2, 2, 1), (9, 2, 1), (16, 2, 1), (17, 2, 1), (16, 32, 16), (17, 32, 16), (9, 32, 2)])
+def test_attention_uncut_tile_order(B, n_q, n_kv, mask):
+    """Masked prompts whose keys are not cut into ranges, of very different lengths and pasts: every tile of every sequence is done,
+    whatever order they are taken in (up to 16 sequences longest first, more in sequence order).  The last: 256-row tiles."""
+    lens = [(i * 97) % 260 for i in range(B)] if n_kv != 2 else [290 - 13 * i for i in range(B)]
+    lens[0] = 300
+    past = [(i * 211) % 200 for i in range(B)]
+    b = Batch(lens, past, 64, n_q, n_kv, seed=73)
+    assert uncut(b) and b.T * (n_q // n_kv) > 128 * B
+    check(attn(b, mask), b, mask=mask)
+    b.pos0[B - 1] = -40                                      # the first 40 tokens see nothing
+    check(attn(b, mask), b, mask=mask)
+    b.pos0[0] = 10 ** 6                                      # far behind every key: all rows see all of them
+    b.kv_len[2 % B] = 0
+    b.table[B // 2, 1] = -1
+    check(attn(b, mask), b, mask=mask)
+
+
+@pytest.mark.parametrize("starts", [[0, 300, 140, 220], [150, 10, 10, 450], [-7, 20, 900, 30], [900, 900, 900, 900], [-1, -1, -1, -1], [450, 0, 450, 0]])
+@pytest.mark.parametrize("mask", [0, 1])
+def test_attention_uncut_prompts_with_starts_that_make_no_sense(starts, mask):
+    b = Batch([150, 150, 150], [20, 70, 40], 16, 4, 2, seed=10)
+    assert uncut(b)
+    b.seq_start = torch.tensor(starts, dtype=torch.int32)
+    guard = torch.full((b.T + 64, b.n_q * D), 7.0, device=DEV, dtype=BF)
+    attn(b, mask, out=guard[32:32 + b.T])
+    assert (guard[:32] == 7).all() and (guard[32 + b.T:] == 7).all()
