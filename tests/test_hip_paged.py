@@ -652,3 +652,36 @@ def test_attention_uncut_prompts_with_starts_that_make_no_sense(starts, mask):
     guard = torch.full((b.T + 64, b.n_q * D), 7.0, device=DEV, dtype=BF)
     attn(b, mask, out=guard[32:32 + b.T])
     assert (guard[:32] == 7).all() and (guard[32 + b.T:] == 7).all()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("lens,past,later,n_q,n_kv,cut", [
+    ([1, 1, 1], [40, 0, 17], [300, 2, 0], 16, 8, False),     # 16-row tiles
+    ([1, 2], [1000, 30], [3000, 5], 4, 2, True),
+    ([16, 9], [100, 31], [60, 200], 6, 2, False),            # 32
+    ([32, 20], [1000, 64], [2000, 900], 4, 2, True),
+    ([100, 90], [64, 0], [64, 300], 4, 2, False),            # 128
+    ([64, 64], [1000, 300], [3000, 0], 8, 2, True),          # a block of 64 at 1000 of 4064 keys
+    ([200, 130], [500, 1500], [2000, 100], 4, 2, True),
+    ([200], [64], [300], 320, 40, False),                    # 256
+    ([60, 40], [1000, 320], [2500, 600], 64, 2, True),
+])
+def test_attention_later_positions(lens, past, later, n_q, n_kv, cut, cache):
+    """The denoiser's step in the middle of a sequence: keys behind the new tokens are in the cache.  Unmasked rows see them, masked ones
+    those of their own block."""
+    b = Batch(lens, [p + x for p, x in zip(past, later)], 16, n_q, n_kv, cache, seed=75, spare_rows=1)
+    b.pos0 -= torch.tensor(later, dtype=torch.int32)
+    assert uncut(b) != cut
+    outs = {}
+    for mask in (0, 1, 32, 64):
+        outs[mask] = attn(b, mask)
+        check(outs[mask], b, mask=mask)
+    # what is not seen: keys from the end of the last token's block on
+    for mask in (1, 64):
+        d = {n: getattr(b, n).clone().to(DEV) for n in ("q", "k", "v", "table", "seq_start", "pos0", "kv_len")}
+        d["kv_len"] = torch.minimum(b.kv_len, (b.pos0 + torch.tensor(lens, dtype=torch.int32) - 1) // mask * mask + mask).to(DEV)
+        less = attn(b, mask, dev=d)
+        torch.cuda.synchronize()
+        n = b.starts[-1]
+        # both within half a step of one value
+        assert (less[:n].float() - outs[mask][:n].float()).norm() <= 2 * 2.0 ** -8 * outs[mask][:n].float().norm()

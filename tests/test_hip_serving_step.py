@@ -50,8 +50,9 @@ class Server:
         self.cos, self.sin = ang.cos().to(BF).to(DEV), ang.sin().to(BF).to(DEV)
         self.adapters = adapters
 
-    def step(self, ids, mask, rewind=0):
-        """ids: new token ids per sequence (lists, may be empty); `rewind`: positions of each sequence that are written anew."""
+    def step(self, ids, mask, rewind=0, keep=False):
+        """ids: new token ids per sequence (lists, may be empty); `rewind`: positions of each sequence that are written anew; `keep`: what
+        lies behind the new tokens stays part of its sequence."""
         e, s = self.eng, _s()
         lens = [len(x) for x in ids]
         starts = [0]
@@ -59,7 +60,7 @@ class Server:
             starts.append(starts[-1] + n)
         T = starts[-1]
         past = [n - rewind for n in self.length]
-        self.length = [p + n for p, n in zip(past, lens)]
+        self.length = [max(p + n, old) if keep else p + n for p, n, old in zip(past, lens, self.length)]
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
         seq, pos0, kv = i32(starts), i32(past), i32(self.length)
         flat = torch.tensor([t for x in ids for t in x], dtype=torch.int64, device=DEV)
@@ -133,6 +134,27 @@ def test_denoise_block_over_kept_keys(engine):
     whole, _ = srv.step(ids, 0)
     again, _ = srv.step([x[lo:lo + n] for x in ids], 0, rewind=L - lo)
     assert rel(again.view(B, n, H), whole.view(B, L, H)[:, lo:lo + n]) < BAND
+
+
+@pytest.mark.parametrize("page", [16, 7])
+def test_denoise_block_with_keys_on_both_sides(engine, page):
+    """A block in the middle, later positions kept: unmasked, the hidden rows of the whole sequence; in blocks of 32, those of the block-causal
+    whole, whatever lies behind."""
+    g = torch.Generator().manual_seed(5)
+    B, L, lo, n = 2, 96, 32, 32
+    ids = torch.randint(0, V - 2, (B, L), generator=g).tolist()
+    block = [x[lo:lo + n] for x in ids]
+    for mask in (0, 32):
+        srv = Server(engine, B, L, page)
+        whole, _ = srv.step(ids, mask)
+        again, _ = srv.step(block, mask, rewind=L - lo, keep=True)
+        assert srv.length == [L] * B
+        assert rel(again.view(B, n, H), whole.view(B, L, H)[:, lo:lo + n]) < BAND
+        short, _ = srv.step(block, mask, rewind=L - lo)          # the same without them
+        if mask:
+            assert rel(short, again) < BAND
+        else:
+            assert rel(short, again) > BAND
 
 
 @pytest.mark.parametrize("page,cache", [(16, _lib.CACHE_BF16), (7, _lib.CACHE_BF16), (64, _lib.CACHE_E4M3)])
