@@ -183,3 +183,45 @@ def test_lora_infinities_and_the_end_of_the_range(rank):
     out[0, :c.N], out[1, :c.N] = c.r[0, :c.N].to(DEV), c.r[1, :c.N].to(DEV)
     c.x[0], c.x[1] = 0, 0
     c.check(out)
+
+
+def plan(c):
+    """(16-token blocks a tile, K ranges, elements of a range, features of a workgroup) of a call in two launches, as lora.hip cuts it."""
+    cus, up = torch.cuda.get_device_properties(0).multi_processor_count, lambda a, b: -(-a // b)
+    mt = 1 if c.T / c.B <= 16 else 2
+    tiles = max(up(c.T, 16 * mt), c.B)
+    nslice = 512 if tiles * up(c.N, 512) >= cus else 256
+    most = (2 * c.K + 4 * c.N) // 8 // (4 * c.rank * (1 + up(c.N, nslice)))
+    ks = max(1, min(max(min(up(4 * cus, tiles), most), up(cus, tiles)), c.K // 256))
+    chunk = up(up(c.K, ks), 64) * 64
+    split = up(c.K, chunk)
+    bytes_ = _lib.load().coda_lora_workspace_bytes(c.T, c.B, c.N, c.K, c.rank)
+    assert bytes_ == (c.T // (16 * mt) + c.B) * 16 + split * c.T * c.rank * 4
+    return mt, split, chunk, nslice
+
+
+def both_places(c):
+    c.check(c.call())
+    out = c.call(in_place=True)
+    c.check(out)
+    assert torch.equal(out[c.live:].cpu(), c.r[c.live:]) and torch.equal(out[:, c.N:].cpu(), c.r[:, c.N:])
+
+
+@pytest.mark.parametrize("rank", [32, 64, 128])
+@pytest.mark.parametrize("K,N", [(1088, 520), (2048, 1056)])
+@pytest.mark.parametrize("most", [16, 40])
+def test_lora_several_steps_of_both_products(most, K, N, rank):
+    """Many tiles: a workgroup of the first launch takes more than two steps of 256 elements of K, one of the second more than one step of
+    256 features, the last of them short; also where it only copies."""
+    lens = [1 + (i * 7) % 16 if most == 16 else 17 + (i * 7) % 24 for i in range(300)]
+    c = Case(lens, [(i * 3) % 5 - 1 for i in range(300)], K, N, rank, seed=rank, pad=8, spare=3)
+    mt, split, chunk, nslice = plan(c)
+    assert mt == (1 if most == 16 else 2) and chunk > 512 and nslice == 512
+    both_places(c)
+
+
+def test_lora_blocks_over_ranges_of_several_steps():
+    """32 blocks of 32 tokens, K 6144 in eight ranges of three steps each."""
+    c = Case([32] * 32, [(i * 3) % 9 - 1 for i in range(32)], 6144, 2048, 64, n=8, seed=3, pad=8)
+    assert plan(c) == (2, 8, 768, 256)
+    both_places(c)
