@@ -201,6 +201,7 @@ extern "C" int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out,
                                  float v_scale, int n_q, int n_kv, float eps, int flags, void* stream) {
     const char* who = "coda_paged_append";
     if (B <= 0 || T <= 0 || n_q <= 0 || n_kv <= 0 || max_pos <= 0) return coda_refuse(who, CODA_ERR_SHAPE, "a size is not positive");
+    if (B > 1 << 30) return coda_refuse(who, CODA_ERR_SHAPE, "B exceeds 2^30");     // the other two have a workgroup per sequence: fewer
     if ((long long)n_q + 2LL * n_kv > MAX_HEADS) return coda_refuse(who, CODA_ERR_SHAPE, "too many heads");
     if (ld_qkv < ((long long)n_q + 2LL * n_kv) * HEAD_DIM || ld_q < (long long)n_q * HEAD_DIM) return coda_refuse(who, CODA_ERR_SHAPE, "a row stride is shorter than a row");
     if (!qkv || !q_out || !cos || !sin || !seq_start || !pos0) return coda_refuse(who, CODA_ERR_ARG, "null pointer");

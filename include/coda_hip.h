@@ -257,7 +257,7 @@ int coda_origin_transfer(long long* x, const long long* x0, const int* dst_pos, 
  * (pos0 int32 [B]), which picks its row of cos / sin (bf16 [max_pos, 128]) and its slot.  q_weight / k_weight bf16 [128], or
  * both NULL: no norm.  q_out bf16 [T, n_q * 128]: the q columns of qkv (in place) or memory apart from qkv.
  * Arithmetic in fp32, rounded once to the stored type (e4m3: times the fp32 reciprocal of the scale, to nearest even,
- * clamped to +-448); flags CODA_APPEND_STEPWISE: bf16 rounding after every operation as coda_qknorm_rope does, so that a cached
+ * clamped to +-448).  B is at most 2^30.  flags CODA_APPEND_STEPWISE: bf16 rounding after every operation as coda_qknorm_rope does, so that a cached
  * key has the bits that the uncached forward computes.  A token whose position is outside [0, max_pos) is skipped whole;
  * one whose page is not there gets its q row only.  Two tokens of one call must not share a slot (which one stays, or which
  * part of either, is not defined). */

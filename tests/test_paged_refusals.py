@@ -104,11 +104,13 @@ def test_attn_workspace_sizes():
     # n_kv * page_size * 128 is 2^64: a page_stride of any length would pass for a page
     ("coda_paged_attn", dict(T=1, n_q=1 << 30, n_kv=1 << 30, ld_q=1 << 38, ld_out=1 << 38, page_size=1 << 27, page_stride=2048), "SHAPE", "heads"),
     ("coda_paged_attn", dict(T=1, n_q=(1 << 20) + 1, n_kv=(1 << 20) + 1, ld_q=1 << 38, ld_out=1 << 38, page_stride=1 << 40), "SHAPE", "heads"),
+    # the search for a token's sequence takes (B + 63) / 64 of them a step
+    ("coda_paged_append", dict(B=(1 << 31) - 1), "SHAPE", "2^30"), ("coda_paged_append", dict(B=(1 << 30) + 1), "SHAPE", "2^30"),
     ("coda_lora_bf16", dict(N=2147483640, ldr=1 << 31, ldc=1 << 31), "SHAPE", "2^30"),
     ("coda_lora_bf16", dict(K=2147483584, ldx=1 << 31), "SHAPE", "2^30"),
 ])
 def test_sizes_whose_sums_would_wrap(name, change, code, words):
-    refused(name, {"coda_paged_attn": ATTN, "coda_lora_bf16": LORA}[name], change, code, words)
+    refused(name, {"coda_paged_append": APPEND, "coda_paged_attn": ATTN, "coda_lora_bf16": LORA}[name], change, code, words)
 
 
 def test_workspaces_of_sizes_that_would_wrap():
