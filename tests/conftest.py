@@ -50,6 +50,15 @@ def full_model():
     return cfg, m
 
 
+@pytest.fixture(scope="module", autouse=True)
+def _no_garbage_of_other_modules():
+    """Tensors that the modules before left in reference cycles (a class made inside a test holds what it closes over until the collector
+    comes by) are freed here, and not in the middle of a test that counts allocations."""
+    import gc
+    gc.collect()
+    yield
+
+
 @pytest.fixture(scope="session", autouse=True)
 def _progress_heartbeat():
     """The full-size parity tests spend minutes inside the CPU oracle without printing; the GPU box takes a command that
