@@ -685,3 +685,21 @@ def test_attention_later_positions(lens, past, later, n_q, n_kv, cut, cache):
         n = b.starts[-1]
         # both within half a step of one value
         assert (less[:n].float() - outs[mask][:n].float()).norm() <= 2 * 2.0 ** -8 * outs[mask][:n].float().norm()
+
+
+def test_attention_of_a_mixed_step_in_two_calls():
+    """Prompts in front, single tokens behind: one call for each kind, the second with its rows, starts and page table from there on."""
+    b = Batch([150, 90] + [1] * 6, [30, 0] + [100 + 90 * i for i in range(6)], 16, 16, 8, seed=77)
+    check_pair(attn(b, 1), b, mask=1)
+    d = {n: getattr(b, n).to(DEV) for n in ("q", "k", "v", "table", "seq_start", "pos0", "kv_len")}
+    out, cut, row, T, B = torch.full((b.T, b.n_q * D), float("nan"), device=DEV, dtype=BF), 2, b.starts[2], b.T, b.B
+    b.T, b.B = row, cut
+    attn(b, 1, dev=d, out=out)
+    first = b.keep
+    late = {n: d[n][cut:] for n in ("table", "pos0", "kv_len")} | {"q": d["q"][row:], "seq_start": d["seq_start"][cut:] - row, "k": d["k"], "v": d["v"]}
+    b.T, b.B = T - row, B - cut
+    attn(b, 1, dev=late, out=out[row:])
+    torch.cuda.synchronize()
+    del first
+    b.T, b.B = T, B
+    check_pair(out, b, mask=1)
