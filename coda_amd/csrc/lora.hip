@@ -8,12 +8,12 @@
 //
 // v_mfma_f32_16x16x32_bf16 in both, weights as the A operand: a lane then holds four consecutive outputs (ranks, features) of one
 // token.  Both are bound by memory at serving ranks (8 .. 128).  X, A, R and C move as contiguous 512 bytes of a row, through LDS:
-// fragments straight from memory (16 rows x 64 B an instruction) took 27 + 120 us where this takes 22 + 95 (15.5 k tokens, rank 32,
-// 2048 -> 6144).  U enters the second product as a bf16 pair (value and remainder): the extra matrix instructions are free in a
+// fragments straight from memory (16 rows x 64 B an instruction) took 27 + 120 us where this took 22 + 95 (17.9 k tokens, rank 32,
+// 2048 -> 6144; later steps took the second to 82).  U enters the second product as a bf16 pair (value and remainder): the extra matrix instructions are free in a
 // kernel that waits for memory, and U keeps 16 bits.
-// Measured: 15.5 k tokens of 32 sequences, rank 32, 2048 -> 6144: down 22 us, up 81, together 517 MB at 5.0 TB/s (a large copy: 5.2); 32
-// blocks of 32 tokens, rank 64, 6144 -> 2048: 7.7 + 7 us, bound by the latency of one tile's chain (tile, slabs, products, result);
-// 32 single tokens, rank 16, 2048 -> 4096, in one launch: 6.7 us.
+// Measured: 17.9 k tokens of 32 sequences, rank 32, 2048 -> 6144: down 22 us, up 82, a call 102: 508 MB at 5.0 TB/s (a large copy: 5.1); 32
+// blocks of 32 tokens, rank 64, 6144 -> 2048: 8.1 + 7.6 us, bound by the latency of one tile's chain (tile, slabs, products, result);
+// 32 single tokens, rank 16, 2048 -> 4096, in one launch: 6.8 us.
 #include "paged_common.h"
 #include <type_traits>
 
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     constexpr int NL = Down<MT, RT>::NL;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Two workgroups share the ranks beyond 64, eight apart, so that they run on one XCD and find X in its L2.  (One with all 128 has a CU to
-    // itself and nothing to run beside its waits: 15.5 k tokens, rank 128, 6144 -> 2048 227 us against 196, 2048 -> 2048 137 against 123.)
+    // itself and nothing to run beside its waits: 17.9 k tokens, rank 128, 6144 -> 2048 227 us against 196, 2048 -> 2048 137 against 123.)
     const bool two = a.rank > 16 * RT;
     const int half = two ? (blockIdx.x >> 3) & 1 : 0, unit = two ? (int)(blockIdx.x >> 4) * 8 + (int)(blockIdx.x & 7) : (int)blockIdx.x;
     const int slot = unit / a.ksplit, ks = unit % a.ksplit, rank0 = half * 16 * RT;

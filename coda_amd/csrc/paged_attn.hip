@@ -87,7 +87,7 @@ __device__ __forceinline__ int keys_of(int kv, int range_keys) {
 // Tile k of a sequence sees about min(kv, pos0 + (k + 1) R / g) keys, which grows with k, so how many of its tiles see at least `keys`
 // is a formula and the order needs no sorting: lane j counts the tiles of at least the j-th of 33 thresholds.  For up to 16 sequences: the
 // search walks over all of them, and tiles of one sequence that run at different times no longer find its keys in the L2 (us with / without:
-// 4 x 2048 tokens 94 / 121, 8 x 2048 179 / 203, 16 x 1000 behind 500 196 / 204, but 30 x 600 125 / 106, 32 x 384 78 / 65).
+// 4 x 2048 tokens 129 / 166, 8 x 2048 238 / 263, 16 x 1000 behind 500 241 / 264, but 30 x 600 131 / 126, 32 x 384 79 / 65).
 constexpr int LONGEST_FIRST = 16, LEVELS = 32;
 
 struct Cost {
@@ -642,10 +642,10 @@ __global__ __launch_bounds__(256, RG == 1 && F8 ? 3 : 2) void paged_attn_few_ker
 // the matrix unit does half as much again), causal 225 us; 2 x 8192 no mask 1419 us = 775 TFLOP/s; a large matrix product reaches 1257 on
 // this card.  One bf16 weight in place of the pair took 291, 175 and 1025 us, with an error of 0.0022 of the result where its own rounding
 // to bf16 is 0.0017: a call's rows would be less exact for being many.
-// With one weight a key were measured: whole bf16 tiles straight to LDS instead of through registers: 8 x 2048 causal 184 / 191 us (one
-// card, in turn), 8 x 200 behind 4000 keys 106 / 117, 16 x 64 behind 2000 54.5 / 57.  Slower or no faster, against 303 .. 314 us for 8 x
-// 2048 without mask through registers: the two halves of the workgroup one barrier apart (341), the softmax of a tile beside the scores of
-// the next (311), wave priorities around the products (316).
+// Whole bf16 tiles straight to LDS instead of through registers: 8 x 2048 no mask 399 / 403 us (another card, in turn, three times), 2 x 8192
+// 1504 / 1526, 8 x 200 causal over 4000 keys 122 / 126.  Tried with one weight, and slower or no faster against 303 .. 314 us for 8 x 2048
+// without mask through registers: the two halves of the workgroup one barrier apart (341), the softmax of a tile beside the scores of the
+// next (311), wave priorities around the products (316).
 constexpr int MANY_TILE = 64;
 constexpr int MANY_BUF = 2 * MANY_TILE * 256;                   // K and V image: 32 KiB
 
@@ -1065,9 +1065,9 @@ Plan make_plan(int T, int B, int max_kv, int n_q, int n_kv, bool slanted, int cu
     const long long slots = p.R == 256 ? cus : two;
     // The shortest range.  Tiles on less than a quarter of the chip wait for latency, and the chain of a range's tiles is what they wait
     // for: 128 keys, once there are enough of them to pay for the second kernel (us uncut / cut into 128 ..: one token on 8 heads, 700 keys
-    // 13.2 / 14.1, 1000 15.6 / 14.4, 1500 19.8 / 14.4, 5000 50 / 15.7; a block of 32 700 17.5 / 16.4, 1500 26 / 17.2; 100 tokens 500 21.2 / 18.5,
-    // 1500 42.5 / 20.2).  Otherwise eight steps of a workgroup, 1024 or 512 keys (us at half / at it / at twice: 32 single tokens x 2000 keys
-    // 53.9 / 50.6 / 50.9, 8 blocks of 128 tokens x 2000 49.8 / 48.5 / 57.3, 8 of 200 x 4000 108 / 101 / 102).  No more partial outputs than
+    // 13.4 / 13.8, 1000 15.9 / 14.7, 1500 19.8 / 14.8, 5000 50 / 15.6; a block of 32 700 17.7 / 16.5, 1500 26 / 17.7; 100 tokens 500 22.1 / 19.8,
+    // 1500 50 / 22.4).  Otherwise eight steps of a workgroup, 1024 or 512 keys (us at half / at it / at twice: 32 single tokens x 2000 keys
+    // 54.2 / 50.7 / 50.6, 8 blocks of 128 tokens x 2000 55.3 / 54.2 / 67.7, 8 of 200 x 4000 123 / 122 / 130).  No more partial outputs than
     // 64 MiB.
     const bool idle = some * n_kv * 4 < slots;
     const int least = idle ? 128 : p.R <= 32 ? 1024 : 512;
@@ -1124,7 +1124,7 @@ extern "C" int coda_paged_attn(const void* q, long long ld_q, void* out, long lo
     a.scale_log2e = scale * (f8 ? k_scale : 1.0f) * 1.4426950408889634f;
     if (!(a.scale_log2e >= 1e-30f && a.scale_log2e <= 1e30f)) return coda_refuse(who, CODA_ERR_ARG, "scale times k_scale is not within [1e-30, 1e30]");
     // With some tokens a sequence, a mask hides up to half of what its tiles would see: us with / without counting that, causal: 1 x 2048 tokens
-    // 53 / 61, 1 x 2048 behind 2000 keys 90 / 105, 2 x 900 behind 1000 49 / 56.  Single tokens have nothing to gain, and the grid for the
+    // 66 / 73, 1 x 2048 behind 2000 keys 112 / 130, 2 x 900 behind 1000 equal.  Single tokens have nothing to gain, and the grid for the
     // shorter ranges costs them (128 x 1 over e4m3 81 / 75).
     a.slanted = mask_block > 0 && T > 4LL * B;
     const Plan p = make_plan(T, B, max_kv, n_q, n_kv, a.slanted, coda_device_cus());

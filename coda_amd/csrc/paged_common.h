@@ -1,6 +1,7 @@
 // What the ragged-batch kernels share: packed token rows cut into sequences by seq_start [B+1], and the geometry of a paged
 // key/value cache.  Everything read from device memory (starts, lengths, page numbers) is clamped or tested before it is
-// used as an index: a wrong entry costs the rows it describes, never an access outside the caller's buffers.
+// used as an index: a wrong entry costs rows (its own; starts that decrease, also others of the call, whose tiles are counted past
+// them), never an access outside the caller's buffers.
 #pragma once
 #include "coda_abi_internal.h"
 

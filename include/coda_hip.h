@@ -257,23 +257,23 @@ int coda_origin_transfer(long long* x, const long long* x0, const int* dst_pos, 
  * (pos0 int32 [B]), which picks its row of cos / sin (bf16 [max_pos, 128]) and its slot.  q_weight / k_weight bf16 [128], or
  * both NULL: no norm.  q_out bf16 [T, n_q * 128]: the q columns of qkv (in place) or memory apart from qkv.
  * Arithmetic in fp32, rounded once to the stored type (e4m3: times the fp32 reciprocal of the scale, to nearest even,
- * clamped to +-448).  B is at most 2^30.  flags CODA_APPEND_STEPWISE: bf16 rounding after every operation as coda_qknorm_rope does, so that a cached
- * key has the bits that the uncached forward computes.  A token whose position is outside [0, max_pos) is skipped whole;
- * one whose page is not there gets its q row only.  Two tokens of one call must not share a slot (which one stays, or which
- * part of either, is not defined). */
+ * clamped to +-448); flags CODA_APPEND_STEPWISE: bf16 rounding after every operation as coda_qknorm_rope does, so that a cached
+ * key has the bits that the uncached forward computes.  B is at most 2^30, n_q + 2 n_kv at most 2^20.  A token whose position is
+ * outside [0, max_pos) is skipped whole; one whose page is not there gets its q row only.  Two tokens of one call must not share a
+ * slot (which one stays, or which part of either, is not defined). */
 int coda_paged_append(const void* qkv, long long ld_qkv, void* q_out, long long ld_q, const void* q_weight,
                       const void* k_weight, const void* cos, const void* sin, int max_pos, const int* seq_start,
                       const int* pos0, int B, int T, const int* page_table, long long ld_table, int max_pages, void* k_cache,
                       void* v_cache, long long page_stride, int num_pages, int page_size, int cache_type, float k_scale,
                       float v_scale, int n_q, int n_kv, float eps, int flags, void* stream);
 
-/* Attention of the new tokens' queries over the cache: out_i = softmax_j(scale q_i . K_j) V, n_q % n_kv == 0, n_kv at most 2^20, from one token a
- * sequence (decode) to whole prompts.  q and out bf16 [T, n_q * 128] (out apart from q and the cache).  Sequence b has
+/* Attention of the new tokens' queries over the cache: out_i = softmax_j(scale q_i . K_j) V, n_q % n_kv == 0, n_kv at most 2^20, from
+ * one token a sequence (decode) to whole prompts.  q and out bf16 [T, n_q * 128] (out apart from q and the cache).  Sequence b has
  * kv_len[b] keys, positions 0 .. kv_len[b]-1 (int32 [B]).  mask_block 0: a token sees all of them, later positions included
  * (the denoiser's attention).  mask_block m > 0: token i sees the keys before the end of its block of m positions,
- * j < ((pos0[b] + i) / m + 1) * m (1: causal).  A token that sees no key, or only scores of -infinity, gets zeros.  Keys a token
- * does not see have no influence on it, whatever their slots hold; a NaN score or an infinity or NaN in V that it does see makes
- * its output (of the feature, for V) non-finite.  The same call has the same bits every time; how the keys are cut and in which
+ * j < ((pos0[b] + i) / m + 1) * m (1: causal), and none at a position below 0.  A token that sees no key, or only scores of
+ * -infinity, gets zeros.  Keys a token does not see have no influence on it, whatever their slots hold; a NaN score or an infinity
+ * or NaN in V that it does see makes its output (of the feature, for V) non-finite.  The same call has the same bits every time; how the keys are cut and in which
  * order parts are added follows from the sizes and all sequences' lengths, so a request's last bits may differ in another batch.
  * max_kv: host-side bound of kv_len, at most max_pages * page_size and 2^30 (keys from max_kv on are not seen): it sizes the launch.
  * Scores, maxima, sums and outputs are fp32; weights enter the second product as a bf16 pair (value and remainder: 16 significant
@@ -292,8 +292,9 @@ int coda_paged_attn(const void* q, long long ld_q, void* out, long long ld_out, 
  * X bf16 [T, K] (the projection's input), R bf16 [T, N] (its output, e.g. of coda_gemm_bf16 CODA_EPI_PLAIN), C bf16 [T, N]: R
  * itself (in place) or memory apart from R and X.  A bf16 [n_adapters, rank, K], B bf16 [n_adapters, N, rank], both dense; scale
  * fp32 [n_adapters] on the device or NULL (1); adapter int32 [B], a value outside [0, n_adapters) means none: C[t] = R[t].
- * rank is a multiple of 8 up to 128 (adapters of smaller rank: zero rows of A), K % 64 == 0, N % 8 == 0, T at most 2^28, N and K at most 2^30.  Both products are summed in
- * fp32 and the result is rounded once; X A^T enters the second one as a bf16 pair (16 significant bits).
+ * rank is a multiple of 8 up to 128 (adapters of smaller rank: zero rows of A), K % 64 == 0, N % 8 == 0, T at most 2^28, N and K
+ * at most 2^30.  Both products are summed in fp32 and the result is rounded once; scale * X A^T enters the second one as a bf16 pair
+ * (value and remainder: 16 significant bits; an infinity stays one).
  * workspace: coda_lora_workspace_bytes(T, B, N, K, rank) bytes, 16-byte aligned, contents irrelevant before and after; calls
  * that may run at the same time need one each. */
 long long coda_lora_workspace_bytes(int T, int B, int N, int K, int rank);
